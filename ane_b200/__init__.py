@@ -127,6 +127,17 @@ SIGNATURES = {
     "ane_ipc_get_handle": (_i32, [_vp, _vp, _vp]),
     "ane_ipc_open_handle": (_i32, [_vp, _vp]),
     "ane_ipc_close_handle": (_i32, [_vp]),
+    "ane_attn_prompt_dev": (_i32, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _f, _vp, _vp, _vp, _vp, _vp, _u32, _vp,
+                                   _vp, _vp]),
+    "ane_attn_decode_workspace_size": (_sz, [_u32, _u32, _u32, _u32]),
+    "ane_attn_decode_dev": (_i32, [_u32, _u32, _u32, _u32, _u32, _f, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _u32, _u32,
+                                   _vp, _vp, _vp, _sz, _vp]),
+    "ane_kv_reserve_dev": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp]),
+    "ane_kv_write_dev": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _vp]),
+    "ane_kv_fork_dev": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp]),
+    "ane_kv_free_dev": (_i32, [_vp, _u32, _vp, _vp]),
+    "ane_kv_copy_pages_dev": (_i32, [_vp, _vp, _u32, _vp, _vp, _vp]),
+    "ane_kv_compact_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "ane_device_timeouts": (_i32, []),
     "ane_kernel_launch_count": (_u64, []),
 }
@@ -489,4 +500,138 @@ def q8_0_gemv(W, x, M: int, K: int, out=None, stream=None, static_weights=False)
         out = torch.empty(M, dtype=torch.float32, device=x.device)
     check(_lib.ane_q8_0_gemv_ex_dev(M, K, x.data_ptr(), W.data_ptr(), out.data_ptr(),
                                     WEIGHTS_STATIC if static_weights else 0, _stream_ptr(stream)))
+    return out
+
+
+# ------------------------------------------------------------------ attention
+class Rows(ctypes.Structure):
+    """ane_rows (include/ane_b200.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_size_t), ("head_stride", ctypes.c_size_t)]
+
+
+class Pages(ctypes.Structure):
+    """ane_pages (include/ane_b200.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_uint32),
+                ("page_tokens", ctypes.c_uint32), ("page_stride", ctypes.c_size_t), ("token_stride", ctypes.c_size_t),
+                ("head_stride", ctypes.c_size_t)]
+
+
+_DTYPES = {}  # torch dtype -> ANE_DTYPE_*
+
+
+def _dtype(t) -> int:
+    if not _DTYPES:
+        torch = _torch()
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise TypeError("expected float32, float16 or bfloat16, got %s" % t.dtype) from None
+
+
+def _rows(name: str, t, heads=None, dim=None) -> Rows:
+    """ane_rows of a CUDA tensor [tokens, heads, dim] whose last dimension is contiguous."""
+    if t.dim() != 3 or not t.is_cuda:
+        raise ValueError("%s must be a CUDA tensor [tokens, heads, dim]" % name)
+    _, h, d = t.shape
+    if (heads is not None and h != heads) or (dim is not None and d != dim):
+        raise ValueError("%s has heads x dim %d x %d, expected %s x %s" % (name, h, d, heads, dim))
+    st, sh, sd = t.stride()
+    if sd != 1 and d > 1:
+        raise ValueError("%s: the last dimension must be contiguous" % name)
+    return Rows(t.data_ptr(), st, sh)
+
+
+def _i32_vector(name: str, t, n=None) -> int:
+    torch = _torch()
+    if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous int32 CUDA vector" % name)
+    if n is not None and t.numel() != n:
+        raise ValueError("%s has %d entries, expected %d" % (name, t.numel(), n))
+    return t.data_ptr()
+
+
+def _output(name: str, out, like, out_dtype, stream):
+    """`out` or a new tensor of like's shape; a new one is kept alive for `stream`."""
+    torch = _torch()
+    if out is None:
+        out = torch.empty(like.shape, dtype=out_dtype or like.dtype, device=like.device)
+        if stream is not None:
+            out.record_stream(stream)
+    elif out.shape != like.shape:
+        raise ValueError("%s must have the shape of q" % name)
+    return out
+
+
+def _lse_ptr(lse, q):
+    if lse is None:
+        return None
+    torch = _torch()
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or not lse.is_cuda:
+        raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, heads]")
+    return lse.data_ptr()
+
+
+def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, lse=None, stream=None):
+    """Causal attention over packed prompts: q [tokens, heads, dim], k and v
+    [tokens, kv_heads, dim] (float16 or bfloat16, any token and head strides of
+    whole 16 bytes), sequence s at rows cu_q[s]:cu_q[s+1] of q and
+    cu_k[s]:cu_k[s+1] of k and v (int32; cu_k defaults to cu_q).  The last query
+    of a sequence sees its last key.  scale defaults to dim ** -0.5; out_dtype
+    may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp."""
+    T, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    if v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("k and v must have one shape and q's dtype")
+    n_seq = cu_q.numel() - 1
+    if n_seq < 0:
+        raise ValueError("cu_q needs n_seq + 1 entries")
+    out = _output("out", out, q, out_dtype, stream)
+    rq, rk, rv, ro = _rows("q", q), _rows("k", k, kv_heads, dim), _rows("v", v), _rows("out", out)
+    check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, k.shape[0],
+                                   dim ** -0.5 if scale is None else float(scale), ctypes.byref(rq), ctypes.byref(rk),
+                                   ctypes.byref(rv), _i32_vector("cu_q", cu_q),
+                                   None if cu_k is None else _i32_vector("cu_k", cu_k, n_seq + 1), _dtype(out),
+                                   ctypes.byref(ro), _lse_ptr(lse, q), _stream_ptr(stream)))
+    return out
+
+
+def attn_decode_workspace(batch: int, heads: int, kv_heads: int, dim: int, device="cuda"):
+    """Workspace for attn_decode calls of up to these sizes on one stream."""
+    torch = _torch()
+    n = int(_lib.ane_attn_decode_workspace_size(batch, heads, kv_heads, dim))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, out=None, out_dtype=None, lse=None,
+                workspace=None, stream=None):
+    """Attention of one new token per sequence over a paged cache: q [batch,
+    heads, dim], one layer's pages k and v [pages, page_tokens, kv_heads, dim],
+    tables int32 [n_slots, max_pages], lens int32 [n_slots], row b of the batch
+    in slot slots[b] (default b).  The first `shared` tokens are the same for the
+    whole batch and are read once, through the pages of row 0's slot."""
+    torch = _torch()
+    B, heads, dim = q.shape
+    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("k and v must be [pages, page_tokens, kv_heads, dim] of one layout and q's dtype")
+    pages, page_tokens, kv_heads, kd = k.shape
+    sp, st, sh, sd = k.stride()
+    if kd != dim or (sd != 1 and dim > 1) or not k.is_cuda or not v.is_cuda:
+        raise ValueError("k and v must be CUDA tensors of q's dim, contiguous in it")
+    if tables.dim() != 2 or tables.dtype != torch.int32 or not tables.is_cuda or not tables.is_contiguous():
+        raise ValueError("tables must be a contiguous int32 CUDA tensor [n_slots, max_pages]")
+    n_slots, max_pages = tables.shape
+    if workspace is None:
+        workspace = attn_decode_workspace(B, heads, kv_heads, dim, q.device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    out = _output("out", out, q, out_dtype, stream)
+    rq, ro = _rows("q", q), _rows("out", out)
+    pg = Pages(k.data_ptr(), v.data_ptr(), pages, page_tokens, sp, st, sh)
+    check(_lib.ane_attn_decode_dev(_dtype(q), B, heads, kv_heads, dim, dim ** -0.5 if scale is None else float(scale),
+                                   ctypes.byref(rq), ctypes.byref(pg), tables.data_ptr(), n_slots, max_pages,
+                                   _i32_vector("lens", lens, n_slots),
+                                   None if slots is None else _i32_vector("slots", slots, B), shared, _dtype(out),
+                                   ctypes.byref(ro), _lse_ptr(lse, q), workspace.data_ptr(), workspace.numel(),
+                                   _stream_ptr(stream)))
     return out

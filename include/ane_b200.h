@@ -430,6 +430,129 @@ int ane_ipc_close_handle(void* base);
 int ane_dense_fused_i8_noalloc_dev(uint32_t M, uint32_t N, uint32_t K, float scale, uint8_t relu,
                                    const float* A, const float* B, float* C, void* stream);
 
+/* ------------------------------------------------ attention and its cache
+ * The products around attention are the matvecs above; these calls are what a
+ * decode loop needs between the QKV and the output projection.  No counterpart
+ * in the reference (its ggml backend leaves attention to ggml).
+ *
+ * Element types.  Queries, keys and values are 16-bit (F16 or BF16, one type
+ * per call); scores, softmax statistics and sums are fp32; a result is rounded
+ * once, to out_dtype (the inputs' type or F32). */
+#define ANE_DTYPE_F32 0u
+#define ANE_DTYPE_F16 1u
+#define ANE_DTYPE_BF16 2u
+/* Rows of tokens x heads x dim: element e of head h of token t is
+ * data[t * token_stride + h * head_stride + e] (strides in elements; data and
+ * strides multiples of 16 bytes). */
+typedef struct ane_rows {
+    void* data;
+    size_t token_stride, head_stride;
+} ane_rows;
+
+/* Causal attention over whole prompts, packed one after another.  Sequence s
+ * holds query tokens cu_q[s] .. cu_q[s+1]-1 and key tokens cu_k[s] ..
+ * cu_k[s+1]-1 (device arrays of n_seq + 1 non-decreasing counts; cu_k NULL:
+ * cu_q).  Its last query sees its last key: query i sees keys 0 .. i + lk - lq.
+ * Query head h reads key/value head h / (heads / kv_heads):
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][hk]) * v[j][hk]
+ * A query that sees no key (lk < lq) gives 0 (and lse -inf).  Rows outside the
+ * sequence are never part of a result, whatever they hold.  lse (NULL to skip)
+ * receives [total_q][heads] natural logarithms of the softmax sums.
+ * dim % 8 == 0, dim <= 128; heads a multiple of kv_heads, at most 64 per
+ * kv_head; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold. */
+int ane_attn_prompt_dev(uint32_t dtype, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                        uint32_t total_q, uint32_t total_k, float scale, const ane_rows* q, const ane_rows* k,
+                        const ane_rows* v, const int32_t* cu_q, const int32_t* cu_k, uint32_t out_dtype,
+                        const ane_rows* out, float* lse, void* stream);
+
+/* A layer's pages: element e of head h of token t of page p is
+ * k[p * page_stride + t * token_stride + h * head_stride + e] (v alike;
+ * strides in elements, everything a multiple of 16 bytes).  page_tokens is a
+ * power of two from 8 to 256. */
+typedef struct ane_pages {
+    const void* k;
+    const void* v;
+    uint32_t pages, page_tokens;
+    size_t page_stride, token_stride, head_stride;
+} ane_pages;
+
+/* Attention of one new token for each of `batch` sequences over a paged cache.
+ * Row b of q / out belongs to slot slots[b] (NULL: b) of tables[n_slots]
+ * [max_pages] and lens[n_slots] (device arrays).  Token j of a slot lies in
+ * page tables[slot][j / page_tokens]; tokens 0 .. lens[slot]-1 are attended to
+ * (none: out 0, lse -inf).  The first `shared` tokens are the caller's promise
+ * to be the same for all sequences: they are read once for the batch, through
+ * the pages of batch row 0's slot (whose row must hold them; with lens shorter
+ * than `shared` a sequence sees only its first lens tokens).  Page numbers
+ * outside the pool are read as page 0.  workspace: 256-byte aligned,
+ * ane_attn_decode_workspace_size bytes, any contents, not shared by calls that
+ * may overlap.  batch <= 1024; dim, heads, kv_heads as for ane_attn_prompt_dev. */
+size_t ane_attn_decode_workspace_size(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim);
+int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, float scale,
+                        const ane_rows* q, const ane_pages* pages, const int32_t* tables, uint32_t n_slots,
+                        uint32_t max_pages, const int32_t* lens, const int32_t* slots, uint32_t shared,
+                        uint32_t out_dtype, const ane_rows* out, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* A key/value cache.  k and v: [layers][pages][page_tokens][heads][dim] of
+ * 16-bit elements (contiguous, 16-byte aligned; dim % 8 == 0, dim <= 128;
+ * page_tokens a power of two, 8 to 256; at most 2^19 pages).  refs[pages]:
+ * readers of each page, 0 = free.  tables[slots][max_pages]: page numbers of
+ * each slot, of which the first ceil(lens[slot] / page_tokens) count.
+ * lens[slots]: tokens.  ctl: one uint32, zero at the start, never reset.
+ * A new cache has refs and lens zero.  All of it is device memory; calls on one
+ * cache are ordered on a stream.  Slots out of range are refused or skipped,
+ * and a slot named twice in one call counts once (the first). */
+typedef struct ane_kv_cache {
+    void* k;
+    void* v;
+    uint32_t dtype, layers, pages, page_tokens, heads, dim;
+    int32_t* refs;
+    int32_t* tables;
+    int32_t* lens;
+    uint32_t slots, max_pages;
+    uint32_t* ctl;
+} ane_kv_cache;
+
+/* Grows slots[i] by counts[i] tokens: new pages, the lowest free ones in the
+ * order of the requests, go to the end of its row.  granted[i] = 1, or 0 for a
+ * request that would pass max_pages or that needs pages which, with those of
+ * all valid requests before it, exceed the free ones; a refused request changes
+ * nothing.  n <= 1024. */
+int ane_kv_reserve_dev(const ane_kv_cache* cache, uint32_t n, const int32_t* slots, const int32_t* counts,
+                       int32_t* granted, void* stream);
+/* Writes rows cu[i] .. cu[i+1]-1 of k and v (F32, rounded to nearest, or the
+ * cache's type) to the last cu[i+1]-cu[i] tokens of slots[i] on one layer (cu
+ * NULL: one row per request).  granted (NULL: all) as ane_kv_reserve_dev left
+ * it: rows of refused requests are dropped.  tokens: rows that k and v hold. */
+int ane_kv_write_dev(const ane_kv_cache* cache, uint32_t layer, uint32_t n, const int32_t* slots, const int32_t* cu,
+                     const int32_t* granted, uint32_t tokens, uint32_t src_dtype, const ane_rows* k,
+                     const ane_rows* v, void* stream);
+/* children[i] (an empty slot) becomes a copy of parents[i]: whole pages gain a
+ * reader, the part page at the end is copied on all layers to the lowest free
+ * page, in the order of the requests.  granted as for ane_kv_reserve_dev (0
+ * also if the child is not empty).  A slot that is a child in this call is
+ * still empty as a parent.  n <= 1024. */
+int ane_kv_fork_dev(const ane_kv_cache* cache, uint32_t n, const int32_t* parents, const int32_t* children,
+                    int32_t* granted, void* stream);
+/* Each slot gives up its pages (one reader less) and is empty; its row's
+ * entries stay as they are.  n <= 1024. */
+int ane_kv_free_dev(const ane_kv_cache* cache, uint32_t n, const int32_t* slots, void* stream);
+/* Page src[i] of `from` to page dst[i] of `to` on all layers (one cache or two
+ * of the same dtype, layers, page_tokens, heads and dim; refs and tables are
+ * the caller's).  No dst may be another pair's src or dst; pairs with a page
+ * number out of range are skipped. */
+int ane_kv_copy_pages_dev(const ane_kv_cache* from, const ane_kv_cache* to, uint32_t n, const int32_t* src,
+                          const int32_t* dst, void* stream);
+/* Moves the pages in use to the lowest page numbers: with L pages in use, the
+ * r-th one at or above L goes to the r-th free page below L.  refs_out[pages]
+ * and tables_out[slots][max_pages] receive the new state (they may be the
+ * cache's own arrays; apart from them, readers can go on with the old state
+ * until they are swapped, since the sources of the moves stay intact).
+ * remap[pages]: each page's new number, -1 if free; *live = L. */
+int ane_kv_compact_dev(const ane_kv_cache* cache, int32_t* refs_out, int32_t* tables_out, int32_t* remap,
+                       int32_t* live, void* stream);
+
 /* ------------------------------------------------------------ diagnostics */
 /* Device-side bounded-wait failures on the current device since the last call
  * (and reset): every kernel wait is bounded (about 2 s) and, when it gives up,

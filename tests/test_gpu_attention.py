@@ -1,0 +1,311 @@
+"""attn_prompt and attn_decode against attention in 64 bits (tests/attn_util.py
+derives the error bound): lengths around the tiles, empty sequences and rows,
+grouped heads, strides, garbage next to the sequences, long caches."""
+import pytest
+import torch
+
+from attn_util import check_rows
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def cu_of(lens, start=0):
+    c = [start]
+    for n in lens:
+        c.append(c[-1] + n)
+    return c
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def prompt_case(ane, lq, lk, heads, kv_heads, dim, dtype, out_dtype=None, layout="fused", spread=1.5, seed=0,
+                want_lse=True):
+    """Sequences between rows of NaN (before the first and after the last)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pad = 3
+    cq, ck = cu_of(lq, pad), cu_of(lk, pad)
+    same = lq == lk
+    nan = float("nan")
+
+    def rows(total, h):
+        if layout == "heads_first":
+            return torch.full((h, total, dim), nan, dtype=dtype, device="cuda").permute(1, 0, 2)
+        return torch.full((total, h, dim), nan, dtype=dtype, device="cuda")
+
+    if layout == "fused" and same:
+        buf = torch.full((cq[-1] + pad, heads + 2 * kv_heads, dim), nan, dtype=dtype, device="cuda")
+        q, k, v = buf[:, :heads], buf[:, heads:heads + kv_heads], buf[:, heads + kv_heads:]
+    else:
+        q, k, v = rows(cq[-1] + pad, heads), rows(ck[-1] + pad, kv_heads), rows(ck[-1] + pad, kv_heads)
+    for t, c, sd in ((q, cq, spread), (k, ck, 1.0), (v, ck, 1.0)):
+        n = c[-1] - pad
+        t[pad:pad + n] = (torch.randn(n, t.shape[1], dim, device="cuda", generator=g) * sd).to(dtype)
+    scale = dim ** -0.5
+    out = torch.full((cq[-1] + pad, heads, dim), 7.0, dtype=out_dtype or dtype, device="cuda")
+    lse = torch.full((cq[-1] + pad, heads), 7.0, device="cuda") if want_lse else None
+    got = ane.attn_prompt(q, k, v, i32(cq), None if same else i32(ck), scale=scale, out=out, lse=lse)
+    assert got is out
+    group = heads // kv_heads
+    for s in range(len(lq)):
+        for h in sorted({0, heads - 1, heads // 2}):
+            visible = torch.arange(lq[s], device="cuda") + 1 + (lk[s] - lq[s])
+            visible = visible.clamp(min=0, max=lk[s])
+            check_rows(out[cq[s]:cq[s + 1], h], dtype, q[cq[s]:cq[s + 1], h], k[ck[s]:ck[s + 1], h // group],
+                       v[ck[s]:ck[s + 1], h // group], scale, visible,
+                       lse[cq[s]:cq[s + 1], h] if want_lse else None)
+    # rows of no sequence are not written
+    assert (out[:pad] == 7.0).all() and (out[cq[-1]:] == 7.0).all()
+    return q, k, v, cq, ck, out
+
+
+@pytest.mark.parametrize("lens", [[1], [2, 1, 1], [0, 5, 0], [63, 64, 65], [127, 128, 129], [255, 256, 257, 0, 31],
+                                  [1000], [513, 77, 300]])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 4, 128, F16), (8, 2, 64, BF16)])
+def test_prompt_lengths(ane, lens, heads, kv_heads, dim, dtype):
+    prompt_case(ane, lens, lens, heads, kv_heads, dim, dtype)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (5, 1), (6, 2), (16, 2), (64, 1), (33, 1)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_groups(ane, heads, kv_heads, dtype):
+    prompt_case(ane, [70, 1, 190], [70, 1, 190], heads, kv_heads, 64, dtype)
+    prompt_case(ane, [131], [131], heads, kv_heads, 128, dtype)
+
+
+@pytest.mark.parametrize("dim", [8, 24, 64, 72, 80, 112, 120, 128])
+@pytest.mark.parametrize("layout", ["fused", "heads_first"])
+def test_prompt_dims_layouts(ane, dim, layout):
+    prompt_case(ane, [140, 9], [140, 9], 4, 2, dim, F16, layout=layout)
+    prompt_case(ane, [140, 9], [140, 9], 4, 2, dim, BF16, layout=layout, out_dtype=F32)
+
+
+@pytest.mark.parametrize("lq,lk", [
+    ([5, 100], [700, 100]),       # a block at the end of a longer history
+    ([130, 64], [131, 1000]),
+    ([300, 40, 7], [10, 0, 8]),   # more queries than keys: the first rows see nothing
+    ([256], [255]),
+    ([1, 1, 1], [129, 1, 512]),
+])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_history_and_empty_rows(ane, lq, lk, dtype):
+    prompt_case(ane, lq, lk, 8, 4, 128, dtype)
+    prompt_case(ane, lq, lk, 2, 2, 64, dtype, out_dtype=F32)
+
+
+def test_prompt_large_scores(ane):
+    """Scores of several hundred: the maximum moves far from tile to tile."""
+    prompt_case(ane, [600], [600], 2, 1, 128, F16, spread=60.0)
+    prompt_case(ane, [600], [600], 2, 1, 128, BF16, spread=200.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_many_small_weights(ane, dtype):
+    """One strong key and thousands of weak ones that together outweigh it."""
+    n, d = 6000, 64
+    k = torch.zeros(n, 1, d, device="cuda", dtype=dtype)
+    k[0, 0, 0] = 12.0
+    v = torch.ones(n, 1, d, device="cuda", dtype=dtype)
+    v[0] = -1.0
+    q = torch.zeros(n, 1, d, device="cuda", dtype=dtype)
+    q[:, 0, 0] = 6.0
+    out = ane.attn_prompt(q, k, v, i32([0, n]), scale=0.125)
+    check_rows(out[:, 0], dtype, q[:, 0], k[:, 0], v[:, 0], 0.125, torch.arange(1, n + 1, device="cuda"))
+
+
+def test_prompt_neighbours_may_hold_anything(ane):
+    """NaN, infinities and the type's lowest value in one sequence leave the others' bits alone."""
+    lens = [37, 90, 128, 5, 200]
+    q, k, v, cq, _, clean = prompt_case(ane, lens, lens, 4, 2, 128, F16, seed=3)
+    for bad in (float("nan"), float("inf"), -65504.0):
+        q2, k2, v2 = q.clone(), k.clone(), v.clone()
+        for t in (q2, k2, v2):
+            t[cq[1]:cq[2]] = bad
+            t[cq[3]:cq[4]] = bad
+        out = ane.attn_prompt(q2, k2, v2, i32(cq), scale=128 ** -0.5)
+        for s in (0, 2, 4):
+            assert torch.equal(out[cq[s]:cq[s + 1]], clean[cq[s]:cq[s + 1]])
+
+
+def test_prompt_batch_invariant_and_repeatable(ane):
+    """A sequence's bits do not depend on what it is packed with, nor on the run."""
+    lens = [300, 17, 411]
+    q, k, v, cq, _, out = prompt_case(ane, lens, lens, 8, 2, 128, BF16, seed=5)
+    again = ane.attn_prompt(q, k, v, i32(cq))
+    assert torch.equal(again[cq[0]:cq[-1]], out[cq[0]:cq[-1]])
+    for s in range(3):
+        a, b = cq[s], cq[s + 1]
+        one = ane.attn_prompt(q[a:b], k[a:b], v[a:b], i32([0, b - a]))
+        assert torch.equal(one, out[a:b])
+
+
+def test_prompt_many_sequences(ane):
+    lens = [(7 * i) % 40 for i in range(1024)]
+    prompt_case(ane, lens[:1024], lens[:1024], 2, 1, 64, F16, want_lse=False)
+
+
+def test_prompt_side_stream_and_graph(ane):
+    lens = [200, 64]
+    q, k, v, cq, _, out = prompt_case(ane, lens, lens, 4, 4, 128, F16, seed=9)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = ane.attn_prompt(q, k, v, i32(cq), stream=side)
+    side.synchronize()
+    assert torch.equal(got[cq[0]:cq[-1]], out[cq[0]:cq[-1]])
+    c, res = i32(cq), torch.zeros_like(out)
+    ane.attn_prompt(q, k, v, c, out=res)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ane.attn_prompt(q, k, v, c, out=res)
+    res.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(res[cq[0]:cq[-1]], out[cq[0]:cq[-1]])
+
+
+# --------------------------------------------------------------------- decode
+def decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype, out_dtype=None, layout="tokens", seed=0,
+                extra_pages=5, first_page=0, want_lse=True, total_pages=None):
+    """lens include the shared tokens.  Everything that belongs to no sequence
+    (page tails, other pages, table entries) is NaN or out of range."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    B = len(lens)
+    full = shared // page
+    prefix = list(range(full))
+    rows, at = [], full
+    for b, n in enumerate(lens):
+        need = -(-max(n, shared if b == 0 else 0) // page)
+        mine = max(0, need - full)
+        rows.append(prefix[:min(need, full)] + list(range(at, at + mine)))
+        at += mine
+    perm = torch.randperm(at + extra_pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    pages = total_pages or at + extra_pages + first_page
+    shape = (pages, kv_heads, page, dim) if layout == "heads" else (pages, page, kv_heads, dim)
+    make = (lambda: torch.empty(shape, dtype=dtype, device="cuda")) if total_pages else \
+        (lambda: torch.full(shape, float("nan"), dtype=dtype, device="cuda"))
+    k, v = make(), make()
+    if layout == "heads":
+        k, v = k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3)
+    width = max(1, max(len(r) for r in rows)) + 1
+    slots = torch.randperm(B + 2, generator=torch.Generator().manual_seed(seed + 1))[:B].tolist()
+    tables = torch.full((B + 2, width), 10 ** 9, dtype=torch.int32)
+    lens_t = torch.full((B + 2,), 10 ** 6, dtype=torch.int32)
+    pk = torch.randn(shared, kv_heads, dim, device="cuda", generator=g).to(dtype)
+    pv = torch.randn(shared, kv_heads, dim, device="cuda", generator=g).to(dtype)
+    q = (torch.randn(B, heads, dim, device="cuda", generator=g) * 1.5).to(dtype)
+    seqs = []
+    for b, n in enumerate(lens):
+        ids = [first_page + perm[r] for r in rows[b]]
+        tables[slots[b], :len(ids)] = torch.tensor(ids, dtype=torch.int32)
+        lens_t[slots[b]] = n
+        hold = max(n, shared if b == 0 else 0)
+        own = max(0, hold - shared)
+        ks = torch.cat([pk, torch.randn(own, kv_heads, dim, device="cuda", generator=g).to(dtype)])[:hold]
+        vs = torch.cat([pv, torch.randn(own, kv_heads, dim, device="cuda", generator=g).to(dtype)])[:hold]
+        for i, p in enumerate(ids):
+            part = min(page, hold - i * page)
+            k[p, :part] = ks[i * page:i * page + part]
+            v[p, :part] = vs[i * page:i * page + part]
+        seqs.append((ks[:n], vs[:n]))
+    scale = dim ** -0.5
+    lse = torch.full((B, heads), 7.0, device="cuda") if want_lse else None
+    out = ane.attn_decode(q, k, v, tables.cuda(), lens_t.cuda(), slots=i32(slots), shared=shared, scale=scale,
+                          out_dtype=out_dtype, lse=lse)
+    group = heads // kv_heads
+    for b in range(B):
+        ks, vs = seqs[b]
+        visible = torch.full((group,), lens[b], device="cuda")
+        for h in range(kv_heads):
+            a, e = h * group, (h + 1) * group
+            check_rows(out[b, a:e], dtype, q[b, a:e], ks[:, h], vs[:, h], scale, visible,
+                       lse[b, a:e] if want_lse else None)
+    return q, k, v, tables.cuda(), lens_t.cuda(), i32(slots), out
+
+
+@pytest.mark.parametrize("lens,shared", [
+    ([1], 0), ([1], 1), ([64], 64), ([65, 64, 63], 0), ([65, 64, 70], 64), ([200, 130, 129, 131], 129),
+    ([300, 0, 257, 1000], 256),       # an empty slot behind a prefix
+    ([50, 20, 0, 64], 64),            # all shorter than the shared tokens, row 0 too
+    ([5000], 0), ([4100, 4097], 4096), ([2000] * 9, 1990),
+])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [(4, 4, 128, 16, F16), (8, 2, 64, 32, BF16)])
+def test_decode_lengths(ane, lens, shared, heads, kv_heads, dim, page, dtype):
+    decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype)
+
+
+@pytest.mark.parametrize("page", [8, 16, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+def test_decode_pages_layouts(ane, page, layout):
+    decode_case(ane, [777, 301, 300, 513], 300, 8, 4, 128, page, F16, layout=layout)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (5, 1), (12, 4), (16, 1), (17, 1), (64, 1), (66, 2)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_decode_groups(ane, heads, kv_heads, dtype):
+    decode_case(ane, [400, 210, 260], 200, heads, kv_heads, 128, 16, dtype)
+    decode_case(ane, [9, 70], 0, heads, kv_heads, 64, 16, dtype)
+
+
+@pytest.mark.parametrize("batch", [2, 15, 16, 17, 33, 64, 65, 130])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 2)])
+def test_decode_batches(ane, batch, heads, kv_heads):
+    lens = [260 + (37 * b) % 200 for b in range(batch)]
+    lens[-1] = 0
+    decode_case(ane, lens, 260, heads, kv_heads, 128, 32, BF16)
+    decode_case(ane, lens, 256, heads, kv_heads, 64, 32, F16, out_dtype=F32)
+
+
+@pytest.mark.parametrize("dim", [8, 24, 72, 80, 120])
+def test_decode_dims(ane, dim):
+    decode_case(ane, [333, 140, 141], 140, 6, 3, dim, 16, F16)
+    decode_case(ane, [333, 140, 141], 140, 6, 3, dim, 16, BF16, out_dtype=F32)
+
+
+def test_decode_shared_equals_unshared(ane):
+    """Reading the prefix once or once per sequence differs by rounding only."""
+    q, k, v, tables, lens, slots, out = decode_case(ane, [700, 650, 901], 640, 8, 2, 128, 16, F16, out_dtype=F32)
+    plain = ane.attn_decode(q, k, v, tables, lens, slots=slots, shared=0, out_dtype=F32)
+    assert (plain - out).abs().max() < 2 * 2.0 ** -11 * 4
+
+
+def test_decode_repeatable_stream_graph(ane):
+    q, k, v, tables, lens, slots, out = decode_case(ane, [1500, 0, 1301, 1290], 1290, 8, 2, 128, 64, BF16)
+    ws = ane.attn_decode_workspace(4, 8, 2, 128)
+    for _ in range(3):
+        ws.random_(0, 255)
+        assert torch.equal(out, ane.attn_decode(q, k, v, tables, lens, slots=slots, shared=1290, workspace=ws))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = ane.attn_decode(q, k, v, tables, lens, slots=slots, shared=1290, stream=side)
+    side.synchronize()
+    assert torch.equal(out, got)
+    res = torch.zeros_like(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ane.attn_decode(q, k, v, tables, lens, slots=slots, shared=1290, workspace=ws, out=res)
+    res.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, res)
+
+
+def test_decode_slot_out_of_range_is_empty(ane):
+    q, k, v, tables, lens, slots, out = decode_case(ane, [70, 33, 64], 0, 2, 2, 64, 16, F16)
+    bad = slots.clone()
+    bad[1], bad[2] = -1, 10 ** 6
+    got = ane.attn_decode(q, k, v, tables, lens, slots=bad)
+    assert torch.equal(got[0], out[0]) and (got[1:] == 0).all()
+
+
+def test_decode_long_cache_offsets(ane):
+    """Pages past 4 GB and past 2^31 elements of a pool."""
+    page, kv_heads, dim = 64, 8, 128
+    per_page = page * kv_heads * dim
+    total = (2 ** 31 + 2 ** 22) // per_page + 64
+    decode_case(ane, [1000, 801], 800, 16, kv_heads, dim, page, F16, total_pages=total, first_page=total - 60)
+
+
+def test_decode_full_batch(ane):
+    decode_case(ane, [100 + b % 40 for b in range(1024)], 96, 2, 1, 64, 16, F16, want_lse=False)
