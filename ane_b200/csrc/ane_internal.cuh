@@ -147,10 +147,13 @@ int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void
                          CUtensorMapSwizzle swizzle);
 
 // 3-D TMA tensor map: dims[0] innermost (elements), strides of dims 1 and 2 in
-// bytes (multiples of 16), box box[0] x box[1] x box[2] elements, zero OOB fill,
-// no swizzle.
+// bytes (multiples of 16), box box[0] x box[1] x box[2] elements, zero OOB fill.
 int encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[3],
-                         const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3]);
+                         const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3],
+                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
+// The same in four dimensions.
+int encode_tensor_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+                         const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
 
 // ------------------------------------------------------- small math helpers
 __host__ __device__ inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }

@@ -289,13 +289,14 @@ __device__ __forceinline__ void store2(void* row, uint32_t c, uint32_t out_dtype
 
 // ------------------------------------------------------------ argument checks
 inline int check_shapes(const char* who, uint32_t dtype, uint32_t out_dtype, uint32_t heads, uint32_t kv_heads,
-                        uint32_t dim) {
+                        uint32_t dim, float scale) {
     const std::string w = who;
     ANE_ARG_CHECK(dtype == ANE_DTYPE_F16 || dtype == ANE_DTYPE_BF16, w + ": dtype must be F16 or BF16");
     ANE_ARG_CHECK(out_dtype == dtype || out_dtype == ANE_DTYPE_F32, w + ": out_dtype must be the inputs' type or F32");
     ANE_ARG_CHECK(dim >= 8 && dim <= 128 && dim % 8 == 0, w + ": dim must be a multiple of 8, 8 to 128");
     ANE_ARG_CHECK(kv_heads > 0 && kv_heads <= 1024 && heads >= kv_heads && heads % kv_heads == 0 && heads / kv_heads <= 64,
                   w + ": heads must be a multiple of kv_heads, at most 64 times as many");
+    ANE_ARG_CHECK(scale > 0.0f && scale <= 1e30f, w + ": scale must be positive");
     return ANE_OK;
 }
 inline int check_rows(const char* who, const ane_rows* r, size_t elem) {

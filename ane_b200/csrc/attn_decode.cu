@@ -282,7 +282,7 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
                                    uint32_t n_slots, uint32_t max_pages, const int32_t* lens, const int32_t* slots,
                                    uint32_t shared, uint32_t out_dtype, const ane_rows* out, float* lse,
                                    void* workspace, size_t workspace_bytes, void* stream) {
-    int rc = attn::check_shapes("attn_decode", dtype, out_dtype, heads, kv_heads, dim);
+    int rc = attn::check_shapes("attn_decode", dtype, out_dtype, heads, kv_heads, dim, scale);
     if (rc) return rc;
     ANE_ARG_CHECK(batch <= kMaxBatch, "attn_decode: at most 1024 sequences");
     ANE_ARG_CHECK(q && pages && tables && lens && out, "attn_decode: NULL pointer");
