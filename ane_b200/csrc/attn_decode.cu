@@ -1,247 +1,678 @@
 // attn_decode.cu -- attention of one new token per sequence over a paged cache
 // whose sequences share a prefix.
 //
-// A key/value head's tokens fall into units: the prefix with all of the batch's
-// query rows (batch x heads of the group, in row tiles), and each sequence's own
-// tokens with its group of rows.  All units' 64-token tiles are laid end to end
-// and cut into equal spans, one per block, so that ragged lengths and a single
-// long sequence load the chip alike.  A block leaves per unit it met an
-// unnormalised (m, l, o); attn_decode_join_kernel adds them per output row, in
-// the order of the tiles, so results do not depend on scheduling.
-#include "attn_core.cuh"
+// Two kinds of work.  The prefix meets all of the batch's query rows (batch x
+// heads of the group, per key/value head); each sequence's own tokens meet only
+// its group of rows.
+//
+// decode_kernel does units of at most 16 rows on mma.sync: the own tokens, and
+// the prefix while the batch has few rows.  It is bound by the bytes of K and V,
+// so all units' 64-token tiles are laid end to end and cut into equal spans, one
+// per block: ragged lengths and a single long sequence load the chip alike.  A
+// producer warp streams a span's tiles through a ring by TMA, across unit
+// boundaries, while four warps compute (each a quarter of a tile's tokens).
+//
+// prefix_kernel does the prefix of a batch with more rows on tcgen05
+// (attn_sm100.cuh), 256 rows against every key tile.
+//
+// Both leave unnormalised partial results (m, l, o); join_kernel adds them per
+// output row in a fixed order, so results do not depend on scheduling.
+#include "attn_sm100.cuh"
 
 namespace ane_b200 {
 namespace {
 using namespace attn;
 
 constexpr uint32_t kMaxBatch = 1024;
-constexpr uint32_t kMaxBlocks = 512;
+constexpr uint32_t kMaxBlocks = 512;   // of decode_kernel
+constexpr uint32_t kBigBlocks = 148;   // of prefix_kernel, about
+constexpr int kTile = 64;              // tokens per key/value tile
+constexpr int kThreads = 160;          // four computing warps and the producer
+constexpr int kJoinThreads = 128;
+constexpr int kUnits = 2;              // units announced ahead
+constexpr int kUnitCost = 1;           // a unit's start and end cost about what a tile does
 
 struct Params {
     uint32_t batch, heads, kv_heads, group, dim, out_dtype;
-    uint32_t shared, prefix_tiles, row_tiles, row_tile;  // row_tile: rows per prefix unit (16 or 64)
-    uint32_t n_slots, max_pages, pages, page_shift;
+    uint32_t shared;         // tokens of the prefix
+    uint32_t prefix_tiles;   // its tiles in decode_kernel (0: none, or prefix_kernel does them)
+    uint32_t prefix_rts, own_rts;    // row tiles (16 rows) of a prefix / own unit
+    uint32_t prefix_rows, own_rows;  // rows of a partial result
+    uint32_t big_splits;     // spans of prefix_kernel (0: not used)
+    uint32_t n_slots, max_pages, pages, page_shift, box_keys;
     float scale2;
     ane_rows q, out;
-    const uint8_t *k, *v;
-    size_t page_stride, token_stride, head_stride;  // bytes
     const int32_t *tables, *lens, *slots;
     float* lse;
-    int32_t* cum;        // [batch + 2]: tiles of sequences before b (per head); [batch + 1]: tiles per block
-    float *po, *pm;      // prefix partials: rows x dim; rows x {m, l}
-    float *so, *sm;      // the sequences' own
-    uint32_t blocks;
+    int32_t* cum;       // [batch + 1] steps of the own units of the sequences before b, per head; then steps per block
+    float *po, *pm;     // prefix partials: rows x dim; rows x {m, l}
+    float *so, *sm;     // the sequences' own
+    int* err;
 };
 
 __device__ __forceinline__ int slot_of(const Params& p, uint32_t b) {
-    const int s = p.slots ? p.slots[b] : (int)b;
+    const int s = p.slots ? __ldcg(p.slots + b) : (int)b;
     return s >= 0 && (uint32_t)s < p.n_slots ? s : -1;
 }
 __device__ __forceinline__ int len_of(const Params& p, uint32_t b) {
     const int s = slot_of(p, b);
-    if (s < 0) return 0;
-    const int64_t cap = (int64_t)p.max_pages << p.page_shift;
-    return (int)min((int64_t)max(p.lens[s], 0), min(cap, (int64_t)0x7fffffff));
+    return s < 0 ? 0 : min(max(__ldcg(p.lens + s), 0), (int)(p.max_pages << p.page_shift));
 }
+// Own tiles start where the box of tokens does that holds the first own one.
+__device__ __forceinline__ int own_base(const Params& p) { return (int)(p.shared & ~(p.box_keys - 1)); }
 __device__ __forceinline__ int own_tiles(const Params& p, int len) {
-    return len > (int)p.shared ? (len - (int)p.shared + kTile - 1) / kTile : 0;
+    return len > (int)p.shared ? (len - own_base(p) + kTile - 1) / kTile : 0;
+}
+// Places of a unit of n tiles on the line that is cut into spans.
+__host__ __device__ __forceinline__ int steps(int tiles) { return tiles > 0 ? tiles + kUnitCost : 0; }
+// {token in page, page} of key j; entries past the row and pages outside the
+// pool are never followed.
+__device__ __forceinline__ int2 page_of(const Params& p, const int32_t* table, int j) {
+    const uint32_t e = min((uint32_t)j >> p.page_shift, p.max_pages - 1);
+    const uint32_t page = (uint32_t)__ldcg(table + e);
+    return make_int2(j & ((1 << p.page_shift) - 1), page < p.pages ? (int)page : 0);
 }
 
-template <typename T, int DP, int MW>
-__device__ void run_unit(const Params& p, uint8_t* smem, uint32_t h, uint32_t b, uint32_t rt, bool prefix, int t0,
-                         int t1, size_t slot) {
-    constexpr int STAGES = DP == 128 ? 3 : 4;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Rows<DP> r;
-    const uint16_t* qrow[2];
-    const int rows = prefix ? (int)(p.batch * p.group) - (int)(rt * p.row_tile) : (int)p.group;
+struct Unit {
+    int prefix, head, b, rt;  // b: sequence (own units); rt: row tile; head -1: no more units
+    int t0, t1;               // tiles
+    int base, lo, kend;       // key of tile 0; keys lo .. kend - 1 count
+    int slot;                 // place of the partial result
+};
+
+template <int DP>
+struct DecodeSmem {
+    static constexpr int kStages = DP == 128 ? 3 : 6;
+    static constexpr int kHalf = kTile * 128;        // 64 tokens x 64 elements
+    static constexpr int kBytes = kTile * DP * 2;    // a K or a V tile
+    uint8_t kv[kStages][2][kBytes];
+    uint8_t q[kUnits][16 * DP * 2];  // query rows of a unit
+    int vis[kUnits][16];             // keys that count for each row, from the unit's lo
+    float2 ml[kStages][4][16];       // {m, l} of each warp's rows
+    int cum[kMaxBatch + 1];          // steps of the own units of the sequences before b, per head
+    Unit unit[kUnits];
+    uint64_t full[kStages], empty[kStages], joined[kStages], unit_full[kUnits], unit_empty[kUnits];
+};
+template <int DP>
+constexpr size_t decode_smem_bytes() {
+    return sizeof(DecodeSmem<DP>) + 1024;
+}
+// two blocks per SM (228 KB, 1 KB of it reserved per block)
+static_assert(2 * (decode_smem_bytes<128>() + 1024) <= 233472 && 2 * (decode_smem_bytes<64>() + 1024) <= 233472, "");
+
+// Byte offset of 16-byte chunk c of token row t in a tile as TMA's 128-byte
+// swizzle lays it out, 64-element halves one after the other.
+__device__ __forceinline__ uint32_t tile_off(uint32_t t, uint32_t c) {
+    return (c >> 3) * (kTile * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
+}
+
+// Query rows: the same with halves of 16 rows.
+__device__ __forceinline__ uint32_t q_off(uint32_t row, uint32_t c) {
+    return (c >> 3) * (16 * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {  // bytes < 16: zero-filled
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// A warp's state of a unit's 16 rows: thread holds rows lane / 4 and lane / 4 + 8.
+template <int DP>
+struct Query {
+    uint32_t q[DP / 16][4];
+    int vis[2];
+};
+template <int DP>
+struct Sums {
+    float o[DP / 8][4];
+    float m[2], l[2];
+};
+
+// One warp: 16 tokens of a tile (rows tok0 .. of shared memory, keys j0 ..
+// counted from the unit's lo).
+template <typename T, int DP>
+__device__ __forceinline__ void tile_step(const Query<DP>& q, Sums<DP>& r, uint32_t ks, uint32_t vs, uint32_t tok0,
+                                          int j0, float scale2) {
+    const uint32_t lane = threadIdx.x & 31, mi = lane >> 3, mr = lane & 7;
+    float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int row = (int)((MW == 1 ? 0 : warp * 16) + lane / 4 + 8 * i);
-        qrow[i] = nullptr;
-        r.vis[i] = 0;
-        if (row < rows) {
-            const uint32_t flat = prefix ? rt * p.row_tile + row : (uint32_t)row;
-            const uint32_t bb = prefix ? flat / p.group : b, g = flat % p.group;
-            qrow[i] = static_cast<const uint16_t*>(p.q.data) + (size_t)bb * p.q.token_stride +
-                      (size_t)(h * p.group + g) * p.q.head_stride;
-            r.vis[i] = len_of(p, bb);
-            if (prefix) r.vis[i] = min(r.vis[i], (int)p.shared);
+    for (int kk = 0; kk < DP / 16; kk++) {
+        uint32_t b[4];
+        ldsm4(ks + tile_off(tok0 + (mi >> 1) * 8 + mr, kk * 2 + (mi & 1)), b);
+        Type<T>::mma(s[0], q.q[kk], b[0], b[1]);
+        Type<T>::mma(s[1], q.q[kk], b[2], b[3]);
+    }
+    const int first = j0 + 2 * (int)(lane & 3);
+    float mx[2] = {kNegInf, kNegInf};
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            // selected, not added: a masked score may be anything, NaN included
+            s[n][j] = (uint32_t)(first + n * 8 + (j & 1)) < (uint32_t)q.vis[j >> 1] ? s[n][j] * scale2 : kNegInf;
+            mx[j >> 1] = fmaxf(mx[j >> 1], s[n][j]);
+        }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+    }
+    // most tiles do not move a maximum
+    if (__any_sync(0xffffffffu, mx[0] > r.m[0] || mx[1] > r.m[1])) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float m = fmaxf(r.m[h], mx[h]), base = m == kNegInf ? 0.0f : m;
+            const float c = exp2_fast(r.m[h] - base);
+            r.m[h] = m;
+            r.l[h] *= c;
+#pragma unroll
+            for (int i = 0; i < DP / 8; i++) {
+                r.o[i][2 * h] *= c;
+                r.o[i][2 * h + 1] *= c;
+            }
         }
     }
-    load_q<DP>(r, qrow[0], qrow[1], p.dim);
-    const int s = slot_of(p, prefix ? 0 : b);
-    const int32_t* table = p.tables + (size_t)max(s, 0) * p.max_pages;
-    const int kend = prefix ? (int)p.shared : len_of(p, b);
-    const int base = prefix ? 0 : (int)p.shared;
-    const uint8_t *kh = p.k + (size_t)h * p.head_stride, *vh = p.v + (size_t)h * p.head_stride;
-    const uint32_t mask = (1u << p.page_shift) - 1u;
-    run_tiles<T, DP, MW, STAGES>(r, smem, t0, t1, base, kend, p.dim, p.scale2,
-                                 [&](int j, const uint8_t*& k, const uint8_t*& v) {
-                                     const uint32_t e = min((uint32_t)j >> p.page_shift, p.max_pages - 1);
-                                     uint32_t page = (uint32_t)table[e];
-                                     if (page >= p.pages) page = 0;
-                                     const size_t off = (size_t)page * p.page_stride + ((uint32_t)j & mask) * p.token_stride;
-                                     k = kh + off;
-                                     v = vh + off;
-                                 });
-    if (MW == 1) join_warps<DP>(r, smem);
-    if (MW == 1 && warp) return;
-    float* o = prefix ? p.po : p.so;
-    float* ml = prefix ? p.pm : p.sm;
-    const int limit = min(rows, prefix ? (int)p.row_tile : (int)p.group);
+    const float off[2] = {Type<T>::kShift - (r.m[0] == kNegInf ? 0.0f : r.m[0]),
+                          Type<T>::kShift - (r.m[1] == kNegInf ? 0.0f : r.m[1])};
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int row = (int)((MW == 1 ? 0 : warp * 16) + lane / 4 + 8 * i);
-        if (row >= limit) continue;
-        const size_t at = slot * (prefix ? p.row_tile : p.group) + row;
-        if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + at * 2) = make_float2(r.m[i], r.l[i]);
+    for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int n = 0; n < DP / 8; n++) {
-            const uint32_t c = n * 8 + 2 * (lane & 3);
-            if (c < p.dim) *reinterpret_cast<float2*>(o + at * p.dim + c) = make_float2(r.o[n][2 * i], r.o[n][2 * i + 1]);
+        for (int j = 0; j < 4; j++) {
+            s[n][j] = exp2_fast(s[n][j] + off[j >> 1]);
+            r.l[j >> 1] += s[n][j];
         }
+    const uint32_t a[4] = {Type<T>::pack(s[0][0], s[0][1]), Type<T>::pack(s[0][2], s[0][3]),
+                           Type<T>::pack(s[1][0], s[1][1]), Type<T>::pack(s[1][2], s[1][3])};
+#pragma unroll
+    for (int n = 0; n < DP / 8; n += 2) {
+        uint32_t b[4];
+        ldsm4_t(vs + tile_off(tok0 + (mi & 1) * 8 + mr, n + (mi >> 1)), b);
+        Type<T>::mma(r.o[n], a, b[0], b[1]);
+        Type<T>::mma(r.o[n + 1], a, b[2], b[3]);
     }
+}
+
+// Word i of this lane's accumulators in the 16 token rows of a stage that only
+// `warp` reads (and has read).  Words 4 x .. 4 x + 3 are column block x of 8.
+template <int DP>
+__device__ __forceinline__ float* spill(uint8_t (*kv)[kTile * DP * 2], int warp, int i) {
+    constexpr int kPerPiece = 16;  // 16 rows x 128 bytes = 16 words per lane
+    const int piece = i / kPerPiece, halves = DP / 64;
+    uint8_t* base = kv[piece / halves] + (piece % halves) * (kTile * 128) + warp * 16 * 128;
+    return reinterpret_cast<float*>(base) + (i % kPerPiece) * 32 + (threadIdx.x & 31);
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int cum[kMaxBatch + 1];
-    ptx::griddep_launch_dependents();
-    ptx::griddep_wait();
-    for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) cum[b] = own_tiles(p, len_of(p, b));
+__global__ void __launch_bounds__(kThreads, 2)
+    decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const Params p) {
+    using S = DecodeSmem<DP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; s++) {
+            ptx::mbar_init(&sm.full[s], 1);
+            ptx::mbar_init(&sm.empty[s], 4);
+            ptx::mbar_init(&sm.joined[s], 4);
+        }
+        for (int u = 0; u < kUnits; u++) {
+            ptx::mbar_init(&sm.unit_full[u], 1);
+            ptx::mbar_init(&sm.unit_empty[u], 4);
+        }
+        ptx::fence_mbarrier_init();
+        ptx::prefetch_tmap(&map_k);
+        ptx::prefetch_tmap(&map_v);
+    }
+    // After prefix_kernel this grid starts when all of that one's blocks have
+    // seen the work before them finished, so the inputs are there (read past L1,
+    // which may hold what they were before); it waits for prefix_kernel itself
+    // only at the end.
+    if (p.big_splits == 0) {
+        ptx::griddep_launch_dependents();
+        ptx::griddep_wait();
+    }
+    for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) sm.cum[b] = steps(own_tiles(p, len_of(p, b)));
     __syncthreads();
-    if (threadIdx.x < 32) {
+    if (warp == 0) {
         int base = 0;
         for (uint32_t b0 = 0; b0 < p.batch; b0 += 32) {
-            const uint32_t b = b0 + threadIdx.x;
-            const int c = b < p.batch ? cum[b] : 0;
+            const uint32_t b = b0 + lane;
+            const int c = b < p.batch ? sm.cum[b] : 0;
             int s = c;
             for (int o = 1; o < 32; o <<= 1) {
                 const int t = __shfl_up_sync(0xffffffffu, s, o);
-                if ((int)threadIdx.x >= o) s += t;
+                if (lane >= o) s += t;
             }
-            if (b < p.batch) cum[b] = base + s - c;
+            if (b < p.batch) sm.cum[b] = base + s - c;
             base += __shfl_sync(0xffffffffu, s, 31);
         }
-        if (threadIdx.x == 0) cum[p.batch] = base;
+        if (lane == 0) sm.cum[p.batch] = base;
     }
     __syncthreads();
-    const int64_t prefix_all = (int64_t)p.prefix_tiles * p.row_tiles * p.kv_heads;
-    const int64_t total = prefix_all + (int64_t)cum[p.batch] * p.kv_heads;
-    const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    const int prefix_steps = steps((int)p.prefix_tiles), prefix_all = prefix_steps * (int)(p.prefix_rts * p.kv_heads);
+    const int per_b = (int)(p.kv_heads * p.own_rts);  // own units of a sequence
+    const int total = prefix_all + sm.cum[p.batch] * per_b;
+    const int per = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
     if (blockIdx.x == 0) {
-        for (uint32_t b = threadIdx.x; b <= p.batch; b += kThreads) p.cum[b] = cum[b];
-        if (threadIdx.x == 0) p.cum[p.batch + 1] = (int32_t)per;
+        for (uint32_t b = threadIdx.x; b <= p.batch; b += kThreads) p.cum[b] = sm.cum[b];
+        if (threadIdx.x == 0) p.cum[p.batch + 1] = per;
     }
-    int64_t at = (int64_t)blockIdx.x * per;
-    const int64_t end = min(at + per, total);
-    while (at < end) {
-        uint32_t h, b = 0, rt = 0;
-        int64_t first;
-        int n;
-        size_t slot;
-        const bool prefix = at < prefix_all;
-        if (prefix) {
-            const uint32_t u = (uint32_t)(at / p.prefix_tiles);
-            h = u / p.row_tiles;
-            rt = u % p.row_tiles;
-            n = (int)p.prefix_tiles;
-            first = (int64_t)u * n;
-            slot = blockIdx.x + u;
-        } else {
-            // cum scaled by kv_heads gives each sequence's first tile; its heads follow one another
-            const int64_t x = at - prefix_all;
-            uint32_t lo = 0, hi = p.batch - 1;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi + 1) >> 1;
-                if ((int64_t)cum[mid] * p.kv_heads <= x) lo = mid; else hi = mid - 1;
-            }
-            b = lo;
-            n = cum[b + 1] - cum[b];
-            h = (uint32_t)((x - (int64_t)cum[b] * p.kv_heads) / n);
-            first = prefix_all + (int64_t)cum[b] * p.kv_heads + (int64_t)h * n;
-            slot = blockIdx.x + (size_t)b * p.kv_heads + h;
-        }
-        const int t0 = (int)(at - first), t1 = (int)min((int64_t)n, end - first);
-        if (prefix && p.row_tile == 64)
-            run_unit<T, DP, 4>(p, smem, h, b, rt, prefix, t0, t1, slot);
-        else if (prefix || p.group <= 16)
-            run_unit<T, DP, 1>(p, smem, h, b, rt, prefix, t0, t1, slot);
-        else
-            run_unit<T, DP, 4>(p, smem, h, b, rt, prefix, t0, t1, slot);
-        at = first + t1;
-    }
-}
+    const int64_t start = (int64_t)blockIdx.x * per;
 
-// One block per (sequence, key/value head): joins the partials of its rows.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const Params p) {
-    ptx::griddep_launch_dependents();
-    ptx::griddep_wait();
-    const uint32_t b = blockIdx.x, h = blockIdx.y;
-    const int64_t per = p.cum[p.batch + 1];
-    const int64_t prefix_all = (int64_t)p.prefix_tiles * p.row_tiles * p.kv_heads;
-    const int n = p.cum[b + 1] - p.cum[b];
-    const int64_t first = prefix_all + (int64_t)p.cum[b] * p.kv_heads + (int64_t)h * n;
-    for (uint32_t g = threadIdx.x / 32; g < p.group; g += kThreads / 32) {
-        const uint32_t flat = b * p.group + g, rt = flat / p.row_tile, lane = threadIdx.x & 31;
-        const uint32_t u = h * p.row_tiles + rt;
-        // spans of blocks that hold partials of this row
-        const int64_t pfirst = (int64_t)u * p.prefix_tiles;
-        const int pc0 = p.prefix_tiles ? (int)(pfirst / per) : 0;
-        const int pc1 = p.prefix_tiles ? (int)((pfirst + p.prefix_tiles - 1) / per) + 1 : 0;
-        const int sc0 = n ? (int)(first / per) : 0, sc1 = n ? (int)((first + n - 1) / per) + 1 : 0;
-        const size_t prow = (size_t)u * p.row_tile + flat % p.row_tile, srow = ((size_t)b * p.kv_heads + h) * p.group + g;
-        float m = kNegInf, l = 0.0f;
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int pass = 0; pass < 2; pass++) {
-            const int c1 = pass ? sc1 : pc1;
-            const float* ml = pass ? p.sm : p.pm;
-            const float* po = pass ? p.so : p.po;
-            const size_t rows = pass ? p.group : p.row_tile, row = pass ? srow : prow;
-            for (int c = pass ? sc0 : pc0; c < c1; c++) {
-                const size_t at = (size_t)c * rows + row;
-                const float2 x = *reinterpret_cast<const float2*>(ml + at * 2);
-                const float mn = fmaxf(m, x.x), base = mn == kNegInf ? 0.0f : mn;
-                const float ca = exp2_fast(m - base), cb = exp2_fast(x.x - base);
-                m = mn;
-                l = l * ca + x.y * cb;
-                if (lane * 4 < p.dim) {
-                    const float4 v = *reinterpret_cast<const float4*>(po + at * p.dim + lane * 4);
-                    o[0] = o[0] * ca + v.x * cb;
-                    o[1] = o[1] * ca + v.y * cb;
-                    o[2] = o[2] * ca + v.z * cb;
-                    o[3] = o[3] * ca + v.w * cb;
+    if (warp == 4) {
+        // --------------------------------------------------------- producer
+        int at = (int)min(start, (int64_t)total);
+        const int end = (int)min(start + per, (int64_t)total);
+        int b_now = -1, len_now = 0;  // the sequence of the last own unit
+        auto next_unit = [&] {  // the unit with the next tile; moves `at` past its part of the span
+            Unit u{};
+            u.head = -1;
+            while (at < end) {
+                int first, n;
+                if (at < prefix_all) {
+                    const int id = at / prefix_steps;
+                    u.prefix = 1;
+                    u.head = id / (int)p.prefix_rts;
+                    u.rt = id % (int)p.prefix_rts;
+                    n = prefix_steps;
+                    first = id * n;
+                    u.slot = (int)blockIdx.x + id;
+                    u.kend = (int)p.shared;
+                } else {
+                    const int x = (at - prefix_all) / per_b;  // cum[b] <= x < cum[b + 1]
+                    int lo = max(b_now, 0), hi = (int)p.batch - 1;
+                    while (lo < hi) {
+                        const int mid = (lo + hi + 1) >> 1;
+                        if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1;
+                    }
+                    if (lo != b_now) len_now = len_of(p, lo), b_now = lo;
+                    u.prefix = 0;
+                    u.b = lo;
+                    n = sm.cum[lo + 1] - sm.cum[lo];
+                    const int id = (at - prefix_all - sm.cum[lo] * per_b) / n;
+                    u.head = id / (int)p.own_rts;
+                    u.rt = id % (int)p.own_rts;
+                    first = prefix_all + sm.cum[lo] * per_b + id * n;
+                    u.slot = (int)blockIdx.x + lo * per_b + id;
+                    u.base = own_base(p);
+                    u.lo = (int)p.shared;
+                    u.kend = len_now;
+                }
+                u.t0 = max(at - first - kUnitCost, 0);
+                u.t1 = min(n, end - first) - kUnitCost;
+                at = first + min(n, end - first);
+                if (u.t1 > u.t0) return u;
+            }
+            u.head = -1;
+            return u;
+        };
+        uint32_t said = 0, n = 0;
+        bool ok = true;
+        // query rows of a unit on their way to its place, which has to be free
+        auto fetch_query = [&](const Unit& u) {
+            const uint32_t e = said % kUnits, rows = u.prefix ? p.batch * p.group : p.group;
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.unit_empty[e], ((said / kUnits) & 1) ^ 1, p.err));
+            if (!ok || u.head < 0) return;
+            constexpr int kChunks = DP / 8;
+#pragma unroll
+            for (int i = 0; i < 16 * kChunks / 32; i++) {
+                const uint32_t row = (uint32_t)(i * 32 + lane) / kChunks, ch = (uint32_t)lane % kChunks;
+                const uint32_t flat = (uint32_t)u.rt * 16 + row;
+                const bool on = flat < rows && ch * 8 < p.dim;
+                const uint32_t b = u.prefix ? flat / p.group : (uint32_t)u.b, g = u.prefix ? flat % p.group : flat;
+                const uint16_t* src = static_cast<const uint16_t*>(p.q.data) +
+                                      (on ? (size_t)b * p.q.token_stride + (size_t)(u.head * p.group + g) * p.q.head_stride + ch * 8 : 0);
+                cp16(ptx::smem_u32(sm.q[e] + q_off(row, ch)), src, on ? 16 : 0);
+            }
+            if (lane < 16) {
+                const uint32_t flat = (uint32_t)u.rt * 16 + lane;
+                sm.vis[e][lane] = flat >= rows ? 0 : u.prefix ? min(len_of(p, flat / p.group), (int)p.shared) : u.kend - u.lo;
+            }
+        };
+        auto announce = [&](const Unit& u) {
+            const uint32_t e = said % kUnits;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                sm.unit[e] = u;
+                ptx::mbar_arrive(&sm.unit_full[e]);
+            }
+            said++;
+        };
+        // one lane per box: K or V, 64 elements, box_keys tokens
+        constexpr int kHalves = DP / 64;
+        const int key_boxes = kTile / (int)p.box_keys, boxes = key_boxes * kHalves;
+        const bool is_v = lane >= boxes, lane_on = lane < 2 * boxes;
+        const int box = is_v ? lane - boxes : lane;
+        const int key0 = box / kHalves * (int)p.box_keys, half = box % kHalves;
+        auto table_of = [&](const Unit& x) {
+            return p.tables + (size_t)max(slot_of(p, x.prefix ? 0 : (uint32_t)x.b), 0) * p.max_pages;
+        };
+        auto entry = [&](const int32_t* table, int j, int kend) {  // page number of this lane's box
+            return lane_on && j < kend ? __ldcg(table + min((uint32_t)j >> p.page_shift, p.max_pages - 1)) : 0;
+        };
+        Unit u = next_unit();
+        const int32_t* table = u.head >= 0 ? table_of(u) : p.tables;
+        int page = u.head >= 0 ? entry(table, u.base + u.t0 * kTile + key0, u.kend) : 0;
+        fetch_query(u);
+        if (ok) announce(u);
+        while (ok && u.head >= 0) {
+            // what the next unit starts with is read while this one loads
+            const Unit following = next_unit();
+            const bool more = following.head >= 0;
+            const int32_t* table_f =
+                !more ? table : following.prefix == u.prefix && following.b == u.b ? table : table_of(following);
+            const int page_f = more ? entry(table_f, following.base + following.t0 * kTile + key0, following.kend) : 0;
+            fetch_query(following);
+            int j = u.base + u.t0 * kTile + key0;
+            for (int t = u.t0; t < u.t1 && ok; t++, j += kTile, n++) {
+                const int page_n = t + 1 < u.t1 ? entry(table, j + kTile, u.kend) : 0;
+                const uint32_t st = n % S::kStages;
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.empty[st], ((n / S::kStages) & 1) ^ 1, p.err));
+                if (!ok) break;
+                // boxes past the last key are left out
+                const int live = min(key_boxes, (u.kend - (u.base + t * kTile) + (int)p.box_keys - 1) / (int)p.box_keys);
+                if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.full[st], 2 * kHalves * 128 * p.box_keys * live);
+                __syncwarp();
+                if (lane_on && j < u.kend)
+                    tma_load_4d(sm.kv[st][is_v] + half * S::kHalf + key0 * 128, is_v ? &map_v : &map_k, &sm.full[st],
+                                half * 64, u.head, j & ((1 << p.page_shift) - 1), (uint32_t)page < p.pages ? page : 0);
+                page = page_n;
+            }
+            if (!ok) break;
+            announce(following);
+            u = following;
+            table = table_f;
+            page = page_f;
+        }
+    } else {
+        // -------------------------------------------------------- computing
+        uint32_t seen = 0, n = 0, join_phase = 0;
+        bool ok = true;
+        while (true) {
+            const uint32_t e = seen % kUnits;
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.unit_full[e], (seen / kUnits) & 1, p.err));
+            if (!ok) break;
+            seen++;
+            const Unit u = sm.unit[e];
+            if (u.head < 0) break;
+            Query<DP> q;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; kk++)
+                ldsm4(ptx::smem_u32(sm.q[e] + q_off((lane >> 3 & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4))), q.q[kk]);
+            q.vis[0] = sm.vis[e][lane / 4];
+            q.vis[1] = sm.vis[e][lane / 4 + 8];
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&sm.unit_empty[e]);
+            Sums<DP> r;
+#pragma unroll
+            for (int i = 0; i < DP / 8; i++) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
+            r.m[0] = r.m[1] = kNegInf;
+            r.l[0] = r.l[1] = 0.0f;
+            uint32_t st = 0;
+            for (int t = u.t0; t < u.t1; t++, n++) {
+                st = n % S::kStages;
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.full[st], (n / S::kStages) & 1, p.err));
+                if (!ok) break;
+                const int j0 = u.base + t * kTile + warp * 16;
+                if (j0 + 16 > u.kend || j0 < u.lo) {
+                    // rows of V that do not count: a weight of 0 does not silence a NaN
+                    for (int i = lane; i < 16 * DP / 8; i += 32) {
+                        const int tok = warp * 16 + i % 16;
+                        const int key = u.base + t * kTile + tok;
+                        if (key >= u.kend || key < u.lo)
+                            *reinterpret_cast<uint4*>(sm.kv[st][1] + tile_off(tok, i / 16)) = make_uint4(0, 0, 0, 0);
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (j0 < u.kend && j0 + 16 > u.lo)
+                    tile_step<T, DP>(q, r, ptx::smem_u32(sm.kv[st][0]), ptx::smem_u32(sm.kv[st][1]), warp * 16,
+                                     j0 - u.lo, p.scale2);
+                __syncwarp();
+                if (t + 1 < u.t1 && lane == 0) ptx::mbar_arrive(&sm.empty[st]);
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 1);
+                r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 2);
+            }
+            // the warps' sums meet in the last tile's stage, which is still theirs;
+            // each warp joins a quarter of the columns
+            constexpr int kQuarter = DP / 8;  // words per lane
+            if ((lane & 3) == 0) {
+                sm.ml[st][warp][lane / 4] = make_float2(r.m[0], r.l[0]);
+                sm.ml[st][warp][lane / 4 + 8] = make_float2(r.m[1], r.l[1]);
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 2; i++) *spill<DP>(sm.kv[st], warp, i) = r.o[i >> 2][i & 3];
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&sm.joined[st]);
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.joined[st], (join_phase >> st) & 1, p.err));
+            if (!ok) break;
+            join_phase ^= 1u << st;
+            float m[2] = {kNegInf, kNegInf}, l[2] = {0.0f, 0.0f}, o[kQuarter];
+            float2 ml[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    ml[h][w] = sm.ml[st][w][lane / 4 + 8 * h];
+                    m[h] = fmaxf(m[h], ml[h][w].x);
+                }
+#pragma unroll
+            for (int i = 0; i < kQuarter; i++) o[i] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                float f[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    f[h] = exp2_fast(ml[h][w].x - (m[h] == kNegInf ? 0.0f : m[h]));
+                    l[h] += ml[h][w].y * f[h];
+                }
+#pragma unroll
+                for (int i = 0; i < kQuarter; i++) o[i] += *spill<DP>(sm.kv[st], w, warp * kQuarter + i) * f[(i & 3) >> 1];
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&sm.empty[st]);
+            float* po = u.prefix ? p.po : p.so;
+            float* pml = u.prefix ? p.pm : p.sm;
+            const int rows = (int)(u.prefix ? p.prefix_rows : p.own_rows);
+            const int limit = min(rows, (int)(u.prefix ? p.batch * p.group : p.group) - u.rt * 16);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = lane / 4 + 8 * h;
+                if (row >= limit) continue;
+                const size_t at = (size_t)u.slot * rows + row;
+                if (warp == 0 && (lane & 3) == 0) *reinterpret_cast<float2*>(pml + at * 2) = make_float2(m[h], l[h]);
+#pragma unroll
+                for (int x = 0; x < kQuarter / 4; x++) {
+                    const uint32_t c = (warp * (kQuarter / 4) + x) * 8 + 2 * (lane & 3);
+                    if (c < p.dim)
+                        *reinterpret_cast<float2*>(po + at * p.dim + c) = make_float2(o[4 * x + 2 * h], o[4 * x + 2 * h + 1]);
                 }
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint8_t* row = static_cast<uint8_t*>(p.out.data) +
-                       ((size_t)b * p.out.token_stride + (size_t)(h * p.group + g) * p.out.head_stride) *
-                           (p.out_dtype == ANE_DTYPE_F32 ? 4 : 2);
-        if (lane * 4 < p.dim) {
-            store2(row, lane * 4, p.out_dtype, l == 0.0f ? 0.0f : o[0] * inv, l == 0.0f ? 0.0f : o[1] * inv);
-            store2(row, lane * 4 + 2, p.out_dtype, l == 0.0f ? 0.0f : o[2] * inv, l == 0.0f ? 0.0f : o[3] * inv);
-        }
-        if (p.lse && lane == 0)
-            p.lse[(size_t)b * p.heads + h * p.group + g] = l == 0.0f ? kNegInf : (m + log2f(l) - Type<T>::kShift) * kLn2;
+    }
+    if (p.big_splits != 0) {
+        ptx::griddep_launch_dependents();
+        ptx::griddep_wait();
     }
 }
 
+// ------------------------------------------------------- prefix on tcgen05
+struct PrefixJob {
+    const Params& p;
+    uint32_t pairs;  // items along the rows: two tiles of 128 / group sequences each
+
+    __device__ void items(BigItem* list) const {
+        const uint32_t lane = threadIdx.x & 31, tt = kBigRows / p.group;
+        const int tiles = (int)((p.shared + kBigKeys - 1) / kBigKeys);
+        for (uint32_t i = threadIdx.x >> 5; i < kMaxItems; i += kBigThreads / 32) {
+            const uint32_t w = i * gridDim.x + blockIdx.x;  // split, head, pair
+            BigItem it{};
+            it.head = -1;
+            if (w < p.big_splits * p.kv_heads * pairs) {
+                const uint32_t split = w / (p.kv_heads * pairs), pair = w % pairs;
+                it.head = (int)(w / pairs % p.kv_heads);
+                it.q_token = (int)(pair * 2 * tt);
+                it.tokens = (int)min(2 * tt, p.batch - pair * 2 * tt);
+                it.lk = (int)p.shared;
+                it.begin = (int)((uint64_t)tiles * split / p.big_splits);
+                const int end = (int)((uint64_t)tiles * (split + 1) / p.big_splits);
+                it.end[0] = end;
+                it.end[1] = it.tokens > (int)tt ? end : it.begin;
+                it.slot = (int)split;
+            }
+            if (lane == 0) list[i] = it;
+        }
+    }
+    __device__ int box_keys() const { return (int)p.box_keys; }
+    __device__ int2 coord(const BigItem& it, int key) const {
+        const int s = slot_of(p, 0);
+        return page_of(p, p.tables + (size_t)max(s, 0) * p.max_pages, min(key, (int)p.shared - 1) & ~((int)p.box_keys - 1));
+    }
+    __device__ int visible(const BigItem& it, int token) const {
+        return min(len_of(p, (uint32_t)(it.q_token + token)), (int)p.shared);
+    }
+    template <int DP>
+    __device__ void finish(const BigItem& it, int t, int row, int token, bool mine, bool any, uint32_t to, float m,
+                           float l, float shift) const {
+        if (!any) return;
+        const size_t rows = (size_t)p.batch * p.group;
+        const size_t at = ((size_t)it.slot * p.kv_heads + it.head) * rows + (size_t)(it.q_token + token) * p.group + row % p.group;
+        if (mine) *reinterpret_cast<float2*>(p.pm + at * 2) = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(to + c, o);
+            ptx::tmem_ld_wait();
+            ptx::pin32(o);
+            if (mine) store32(reinterpret_cast<uint8_t*>(p.po + at * p.dim), c, p.dim, ANE_DTYPE_F32, o, 1.0f);
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBigThreads, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const Params p, uint32_t pairs) {
+    PrefixJob job{p, pairs};
+    big_attention<T, DP>(&map_q, &map_k, &map_v, p.group, p.scale2, p.err, job);
+}
+
+// -------------------------------------------------------------------- join
+// One block per output row; its warps take the partial results in turn.
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
+    __shared__ float sm_m[4], sm_l[4], sm_o[4][128];
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const uint32_t b = blockIdx.x, head = blockIdx.y, h = head / p.group, g = head % p.group;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per = __ldcg(p.cum + p.batch + 1), c0 = __ldcg(p.cum + b), n = __ldcg(p.cum + b + 1) - c0;
+    // spans [pc, pe) and [oc, oe) of blocks hold partials of this row: of span c
+    // at row prow + c * pstep, orow + c * ostep
+    int pc = 0, pe = 0, oc = 0, oe = 0;
+    size_t prow = 0, pstep = 0;
+    const uint32_t flat = b * p.group + g;
+    if (p.big_splits) {
+        pe = (int)p.big_splits;
+        const size_t rows = (size_t)p.batch * p.group;
+        prow = (size_t)h * rows + flat;
+        pstep = rows * p.kv_heads;
+    } else if (p.prefix_tiles) {
+        const int id = (int)(h * p.prefix_rts + flat / 16), first = id * steps((int)p.prefix_tiles);
+        pc = (first + kUnitCost) / per;
+        pe = (first + steps((int)p.prefix_tiles) - 1) / per + 1;
+        prow = (size_t)id * p.prefix_rows + flat % 16;
+        pstep = p.prefix_rows;
+    }
+    const int per_b = (int)(p.kv_heads * p.own_rts), id = (int)(h * p.own_rts + g / 16);
+    const size_t orow = (size_t)((int)b * per_b + id) * p.own_rows + g % 16, ostep = p.own_rows;
+    if (n) {
+        const int first = steps((int)p.prefix_tiles) * (int)(p.prefix_rts * p.kv_heads) + c0 * per_b + id * n;
+        oc = (first + kUnitCost) / per;
+        oe = (first + n - 1) / per + 1;
+    }
+    float m = kNegInf, l = 0.0f;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool on = (uint32_t)lane * 4 < p.dim;
+    // four partials of each warp on their way at a time
+    const int count = (pe - pc) + (oe - oc);
+    for (int i0 = warp; i0 < count; i0 += 16) {
+        float2 x[4];
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + 4 * k;
+            const bool pre = i < pe - pc;
+            const size_t at = pre ? prow + (size_t)(pc + i) * pstep : orow + (size_t)(oc + i - (pe - pc)) * ostep;
+            x[k] = make_float2(kNegInf, 0.0f);
+            v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < count) {
+                x[k] = __ldcg(reinterpret_cast<const float2*>((pre ? p.pm : p.sm) + at * 2));
+                if (on) v[k] = __ldcg(reinterpret_cast<const float4*>((pre ? p.po : p.so) + at * p.dim + lane * 4));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float mn = fmaxf(m, x[k].x), base = mn == kNegInf ? 0.0f : mn;
+            const float ca = exp2_fast(m - base), cb = exp2_fast(x[k].x - base);
+            m = mn;
+            l = l * ca + x[k].y * cb;
+            o[0] = o[0] * ca + v[k].x * cb;
+            o[1] = o[1] * ca + v[k].y * cb;
+            o[2] = o[2] * ca + v[k].z * cb;
+            o[3] = o[3] * ca + v[k].w * cb;
+        }
+    }
+    if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
+    *reinterpret_cast<float4*>(&sm_o[warp][lane * 4]) = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    const uint32_t c = threadIdx.x;
+    m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+    const float base = m == kNegInf ? 0.0f : m;
+    float sum = 0.0f;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float f = exp2_fast(sm_m[w] - base);
+        l += sm_l[w] * f;
+        sum += sm_o[w][c] * f;
+    }
+    if (c < p.dim) {
+        const float y = l == 0.0f ? 0.0f : sum / l;
+        const size_t at = (size_t)b * p.out.token_stride + (size_t)head * p.out.head_stride + c;
+        if (p.out_dtype == ANE_DTYPE_F32)
+            static_cast<float*>(p.out.data)[at] = y;
+        else
+            static_cast<uint16_t*>(p.out.data)[at] = (uint16_t)Type<T>::pack(y, 0.0f);
+    }
+    if (p.lse && c == 0) p.lse[(size_t)b * p.heads + head] = l == 0.0f ? kNegInf : (m + log2f(l) - Type<T>::kShift) * kLn2;
+}
+
+// ------------------------------------------------------------------ launch
 struct Layout {
-    uint32_t row_tile, row_tiles;
+    uint32_t prefix_rts, own_rts, prefix_rows, own_rows, pairs, big_splits;
     size_t cum, pm, po, sm, so, bytes;
 };
 Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
     Layout l;
     const uint32_t group = heads / kv_heads;
     const size_t rows = (size_t)batch * group;
-    l.row_tile = rows <= 16 ? 16 : 64;
-    l.row_tiles = (uint32_t)ceil_div(rows, l.row_tile);
-    const size_t prefix_rows = (kMaxBlocks + (size_t)kv_heads * l.row_tiles) * l.row_tile;
-    const size_t own_rows = (kMaxBlocks + (size_t)batch * kv_heads) * group;
+    l.prefix_rts = (uint32_t)ceil_div(rows, 16);
+    l.own_rts = (uint32_t)ceil_div(group, 16);
+    l.prefix_rows = (uint32_t)(rows < 16 ? rows : 16);
+    l.own_rows = group < 16 ? group : 16;
+    l.pairs = (uint32_t)ceil_div(batch, 2 * (kBigRows / group));
+    l.big_splits = kBigBlocks / (kv_heads * l.pairs);
+    if (l.big_splits == 0) l.big_splits = 1;
+    const size_t prefix_small = (kMaxBlocks + (size_t)kv_heads * l.prefix_rts) * l.prefix_rows;
+    const size_t prefix_big = (size_t)l.big_splits * kv_heads * rows;
+    const size_t prefix_rows = prefix_small > prefix_big ? prefix_small : prefix_big;
+    const size_t own_rows = (kMaxBlocks + (size_t)batch * kv_heads * l.own_rts) * l.own_rows;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -258,13 +689,23 @@ Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
 }
 
 template <typename T, int DP>
-int launch(const Params& p, cudaStream_t s) {
-    static std::atomic<uint64_t> done{0};
-    constexpr int smem = (DP == 128 ? 3 : 4) * 2 * tile_bytes<DP>();
-    int rc = set_max_dynamic_smem(decode_kernel<T, DP>, smem, done);
-    if (rc) return rc;
-    if ((rc = launch_pdl(decode_kernel<T, DP>, dim3(p.blocks), dim3(kThreads), smem, s, p))) return rc;
-    return launch_pdl(decode_join_kernel<T>, dim3(p.batch, p.kv_heads), dim3(kThreads), 0, s, p);
+int launch(const CUtensorMap (&map)[3], const Params& p, uint32_t pairs, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0}, done_big{0};
+    int rc;
+    if (p.big_splits) {
+        if ((rc = set_max_dynamic_smem(prefix_kernel<T, DP>, (int)big_smem_bytes<DP>(), done_big))) return rc;
+        const uint64_t items = (uint64_t)p.big_splits * p.kv_heads * pairs;
+        uint64_t blocks = items < (uint64_t)num_sms() ? items : (uint64_t)num_sms();
+        if (blocks * kMaxItems < items) blocks = ceil_div(items, kMaxItems);
+        if ((rc = launch_pdl(prefix_kernel<T, DP>, dim3((uint32_t)blocks), dim3(kBigThreads), big_smem_bytes<DP>(), s,
+                             map[0], map[1], map[2], p, pairs)))
+            return rc;
+    }
+    if ((rc = set_max_dynamic_smem(decode_kernel<T, DP>, (int)decode_smem_bytes<DP>(), done))) return rc;
+    const uint32_t blocks = (uint32_t)num_sms() * 2 < kMaxBlocks ? (uint32_t)num_sms() * 2 : kMaxBlocks;
+    if ((rc = launch_pdl(decode_kernel<T, DP>, dim3(blocks), dim3(kThreads), decode_smem_bytes<DP>(), s, map[1], map[2], p)))
+        return rc;
+    return launch_pdl(join_kernel<T>, dim3(p.batch, p.heads), dim3(kJoinThreads), 0, s, p);
 }
 
 }  // namespace
@@ -273,7 +714,8 @@ int launch(const Params& p, cudaStream_t s) {
 using namespace ane_b200;
 
 extern "C" size_t ane_attn_decode_workspace_size(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
-    if (kv_heads == 0 || heads < kv_heads || heads % kv_heads || batch > kMaxBatch) return 0;
+    if (kv_heads == 0 || heads < kv_heads || heads % kv_heads || heads / kv_heads > 64 || batch == 0 || batch > kMaxBatch)
+        return 0;
     return layout(batch, heads, kv_heads, dim).bytes;
 }
 
@@ -298,9 +740,12 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
                       (uintptr_t)pages->v % 16 == 0 && pages->page_stride % 8 == 0 && pages->token_stride % 8 == 0 &&
                       pages->head_stride % 8 == 0,
                   "attn_decode: pages must be 16-byte aligned with strides of whole 16 bytes");
-    ANE_ARG_CHECK((uint64_t)max_pages * pt <= 0x7fffff00u, "attn_decode: at most 2^31 tokens per slot");
-    ANE_ARG_CHECK(shared <= (uint64_t)max_pages * pt, "attn_decode: shared exceeds max_pages pages");
     const Layout l = layout(batch, heads, kv_heads, dim);
+    const uint64_t most = (uint64_t)max_pages * pt;  // tokens of a slot
+    ANE_ARG_CHECK(most <= 0x7fffff00u &&
+                      (most / kTile + 3) * kv_heads * ((uint64_t)batch * l.own_rts + l.prefix_rts) <= 0x7fffffffu,
+                  "attn_decode: more than 2^31 tiles of 64 tokens");
+    ANE_ARG_CHECK(shared <= most, "attn_decode: shared exceeds max_pages pages");
     ANE_ARG_CHECK(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= l.bytes,
                   "attn_decode: workspace must be 256-byte aligned and of ane_attn_decode_workspace_size bytes");
     if ((rc = require_sm100())) return rc;
@@ -308,24 +753,42 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     Params p{};
     p.batch = batch, p.heads = heads, p.kv_heads = kv_heads, p.group = heads / kv_heads, p.dim = dim;
     p.out_dtype = out_dtype;
-    p.shared = shared, p.prefix_tiles = (uint32_t)ceil_div(shared, attn::kTile);
-    p.row_tiles = l.row_tiles, p.row_tile = l.row_tile;
+    p.shared = shared;
+    const bool big = shared > 0 && (size_t)batch * p.group > 16;
+    if (big) {
+        const uint32_t tiles = (uint32_t)ceil_div(shared, kBigKeys);
+        p.big_splits = l.big_splits < tiles ? l.big_splits : tiles;
+    } else {
+        p.prefix_tiles = (uint32_t)ceil_div(shared, kTile);
+    }
+    p.prefix_rts = l.prefix_rts, p.own_rts = l.own_rts, p.prefix_rows = l.prefix_rows, p.own_rows = l.own_rows;
     p.n_slots = n_slots, p.max_pages = max_pages, p.pages = pages->pages;
     while ((1u << p.page_shift) < pt) p.page_shift++;
     p.scale2 = scale * attn::kLog2e;
     p.q = *q, p.out = *out;
-    p.k = static_cast<const uint8_t*>(pages->k), p.v = static_cast<const uint8_t*>(pages->v);
-    p.page_stride = pages->page_stride * 2, p.token_stride = pages->token_stride * 2, p.head_stride = pages->head_stride * 2;
     p.tables = tables, p.lens = lens, p.slots = slots, p.lse = lse;
     p.cum = reinterpret_cast<int32_t*>(ws + l.cum);
     p.pm = reinterpret_cast<float*>(ws + l.pm), p.po = reinterpret_cast<float*>(ws + l.po);
     p.sm = reinterpret_cast<float*>(ws + l.sm), p.so = reinterpret_cast<float*>(ws + l.so);
-    // two blocks per SM fit (96 KB of tiles each)
-    p.blocks = (uint32_t)num_sms() * 2 < kMaxBlocks ? (uint32_t)num_sms() * 2 : kMaxBlocks;
+    p.err = device_timeout_flag();
+    // one box shape for both kernels: a page, or 64 tokens of a larger one
+    p.box_keys = pt < (uint32_t)kTile ? pt : (uint32_t)kTile;
+    const auto type = dtype == ANE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    CUtensorMap map[3];
+    if (big && (rc = encode_tensor_map_3d(&map[0], type, q->data, {dim, heads, batch},
+                                          {q->head_stride * 2, q->token_stride * 2}, {64, p.group, 128 / p.group},
+                                          CU_TENSOR_MAP_SWIZZLE_128B)))
+        return rc;
+    const void* pool[2] = {pages->k, pages->v};
+    for (int i = 0; i < 2; i++)
+        if ((rc = encode_tensor_map_4d(&map[1 + i], type, pool[i], {dim, kv_heads, pt, pages->pages},
+                                       {pages->head_stride * 2, pages->token_stride * 2, pages->page_stride * 2},
+                                       {64, 1, p.box_keys, 1}, CU_TENSOR_MAP_SWIZZLE_128B)))
+            return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == ANE_DTYPE_F16)
-        rc = dim <= 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
+        rc = dim <= 64 ? launch<__half, 64>(map, p, l.pairs, s) : launch<__half, 128>(map, p, l.pairs, s);
     else
-        rc = dim <= 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+        rc = dim <= 64 ? launch<__nv_bfloat16, 64>(map, p, l.pairs, s) : launch<__nv_bfloat16, 128>(map, p, l.pairs, s);
     return rc ? rc : ok();
 }

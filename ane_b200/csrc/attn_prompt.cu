@@ -114,10 +114,7 @@ struct PromptJob {
         }
     }
     __device__ int box_keys() const { return kBigKeys; }
-    __device__ void load_box(const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int x, const BigItem& it,
-                             int key) const {
-        tma_load_4d(dst, map, bar, x, it.head, it.k0 + key, 0);
-    }
+    __device__ int2 coord(const BigItem& it, int key) const { return make_int2(it.k0 + key, 0); }
     __device__ int visible(const BigItem& it, int token) const { return max(0, min(it.lk, it.see + token + 1)); }
 
     template <int DP>

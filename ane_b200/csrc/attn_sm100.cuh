@@ -74,8 +74,8 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
 
 // The kernel's frame.  Job supplies:
 //   items(sm.items)             all warps: this block's items, ended by head -1
-//   load_box(map, dst, bar, x, item, key, box)  keys key .. of a tile, one box
-//   kBoxKeys()                  keys per box (a multiple of 8 that divides 128)
+//   box_keys()                  keys per TMA box (a multiple of 8 that divides 128)
+//   coord(item, key)            {token, page} coordinates of the box that starts at a key
 //   visible(item, token)        keys that query token `token` of the item sees
 //   finish(item, t, token, row, tmem_o, m, l)   one thread per row
 template <typename T, int DP, class Job>
@@ -87,7 +87,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
     S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int kBoxes = DP / 64;  // 64-element boxes of 128 rows x 128 bytes
     constexpr int kBoxBytes = 128 * 128;
-    constexpr float kShift = Type<T>::kShift > 0.0f ? 6.0f : 0.0f;
+    constexpr float kShift = Type<T>::kShift;  // with kSlack: F16 weights stay below 2^14
     constexpr bool kBf16 = Type<T>::kShift == 0.0f;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile_tokens = kBigRows / (int)group;
@@ -114,8 +114,10 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
         ptx::tmem_alloc(&sm.tmem, 512);
         ptx::tmem_relinquish();
     }
-    ptx::griddep_launch_dependents();
+    // in this order: a dependent grid that does not wait may still rely on the
+    // work before this one (attn_decode.cu)
     ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
     job.items(sm.items);
     ptx::tc_fence_before();
     __syncthreads();
@@ -124,9 +126,12 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
 
     if (warp >= 8) {
         ptx::regs_dec<88>();
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
             // ---------------------------------------------------------- loads
-            const int box_keys = job.box_keys();
+            // one lane per box: 64 elements x box_keys keys
+            const int box_keys = job.box_keys(), boxes = kBigKeys / box_keys * kBoxes;
+            const int key0 = lane / kBoxes * box_keys, x0 = lane % kBoxes * 64;
+            const uint32_t dst0 = lane % kBoxes * kBoxBytes + key0 * 128;
             uint32_t n = 0, used = 0;
             bool ok = true;
             for (int i = 0; i < kMaxItems && ok; i++) {
@@ -134,26 +139,31 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 if (it.head < 0) break;
                 const int end = max(it.end[0], it.end[1]);
                 if (end <= it.begin) continue;
-                if (!ptx::mbar_wait(&sm.q_empty, (used & 1) ^ 1, err)) break;
+                int2 at = lane < boxes ? job.coord(it, it.begin * kBigKeys + key0) : make_int2(0, 0);
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.q_empty, (used & 1) ^ 1, err));
+                if (!ok) break;
                 used++;
-                const uint32_t q_bytes = kBoxes * 128u * group * tile_tokens;
-                ptx::mbar_arrive_expect_tx(&sm.q_full, q_bytes * ((it.end[0] > it.begin) + (it.end[1] > it.begin)));
-                for (int t = 0; t < 2; t++)
-                    for (int b = 0; b < kBoxes && it.end[t] > it.begin; b++)
-                        ptx::tma_load_3d(sm.q[t] + b * kBoxBytes, map_q, &sm.q_full, b * 64, it.head * (int)group,
-                                         it.q_token + t * tile_tokens);
+                if (lane == 0) {
+                    const uint32_t q_bytes = kBoxes * 128u * group * tile_tokens;
+                    ptx::mbar_arrive_expect_tx(&sm.q_full, q_bytes * ((it.end[0] > it.begin) + (it.end[1] > it.begin)));
+                    for (int t = 0; t < 2; t++)
+                        for (int b = 0; b < kBoxes && it.end[t] > it.begin; b++)
+                            ptx::tma_load_3d(sm.q[t] + b * kBoxBytes, map_q, &sm.q_full, b * 64, it.head * (int)group,
+                                             it.q_token + t * tile_tokens);
+                }
                 for (int j = it.begin; j < end && ok; j++) {
+                    const int2 next = lane < boxes && j + 1 < end ? job.coord(it, (j + 1) * kBigKeys + key0) : at;
                     for (int kv = 0; kv < 2; kv++, n++) {
                         const int st = n % S::kStages;
-                        if (!(ok = ptx::mbar_wait(&sm.kv_empty[st], ((n / S::kStages) & 1) ^ 1, err))) break;
+                        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.kv_empty[st], ((n / S::kStages) & 1) ^ 1, err));
+                        if (!ok) break;
                         const bool tail = kv && (j + 1) * kBigKeys > it.lk;
                         uint64_t* bar = tail ? &sm.tail_full[st] : &sm.kv_full[st];
-                        ptx::mbar_arrive_expect_tx(bar, kBoxes * kBoxBytes);
-                        for (int key = 0; key < kBigKeys; key += box_keys)
-                            for (int b = 0; b < kBoxes; b++)
-                                job.load_box(kv ? map_v : map_k, sm.kv[st] + b * kBoxBytes + key * 128, bar, b * 64, it,
-                                             j * kBigKeys + key);
+                        if (lane == 0) ptx::mbar_arrive_expect_tx(bar, kBoxes * kBoxBytes);
+                        __syncwarp();
+                        if (lane < boxes) tma_load_4d(sm.kv[st] + dst0, kv ? map_v : map_k, bar, x0, it.head, at.x, at.y);
                     }
+                    at = next;
                 }
             }
         } else if (warp == 9 && lane == 0) {
