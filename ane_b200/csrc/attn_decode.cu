@@ -506,27 +506,24 @@ struct PrefixJob {
     const Params& p;
     uint32_t pairs;  // items along the rows: two tiles of 128 / group sequences each
 
-    __device__ void items(BigItem* list) const {
-        const uint32_t lane = threadIdx.x & 31, tt = kBigRows / p.group;
+    __device__ BigItem item(int i) const {
+        const uint32_t tt = kBigRows / p.group, w = (uint32_t)i * gridDim.x + blockIdx.x;  // split, head, pair
         const int tiles = (int)((p.shared + kBigKeys - 1) / kBigKeys);
-        for (uint32_t i = threadIdx.x >> 5; i < kMaxItems; i += kBigThreads / 32) {
-            const uint32_t w = i * gridDim.x + blockIdx.x;  // split, head, pair
-            BigItem it{};
-            it.head = -1;
-            if (w < p.big_splits * p.kv_heads * pairs) {
-                const uint32_t split = w / (p.kv_heads * pairs), pair = w % pairs;
-                it.head = (int)(w / pairs % p.kv_heads);
-                it.q_token = (int)(pair * 2 * tt);
-                it.tokens = (int)min(2 * tt, p.batch - pair * 2 * tt);
-                it.lk = (int)p.shared;
-                it.begin = (int)((uint64_t)tiles * split / p.big_splits);
-                const int end = (int)((uint64_t)tiles * (split + 1) / p.big_splits);
-                it.end[0] = end;
-                it.end[1] = it.tokens > (int)tt ? end : it.begin;
-                it.slot = (int)split;
-            }
-            if (lane == 0) list[i] = it;
+        BigItem it{};
+        it.head = -1;
+        if (w < p.big_splits * p.kv_heads * pairs) {
+            const uint32_t split = w / (p.kv_heads * pairs), pair = w % pairs;
+            it.head = (int)(w / pairs % p.kv_heads);
+            it.q_token = (int)(pair * 2 * tt);
+            it.tokens = (int)min(2 * tt, p.batch - pair * 2 * tt);
+            it.lk = (int)p.shared;
+            it.begin = (int)((uint64_t)tiles * split / p.big_splits);
+            const int end = (int)((uint64_t)tiles * (split + 1) / p.big_splits);
+            it.end[0] = end;
+            it.end[1] = it.tokens > (int)tt ? end : it.begin;
+            it.slot = (int)split;
         }
+        return it;
     }
     __device__ int box_keys() const { return (int)p.box_keys; }
     __device__ int2 coord(const BigItem& it, int key) const {
@@ -536,22 +533,16 @@ struct PrefixJob {
     __device__ int visible(const BigItem& it, int token) const {
         return min(len_of(p, (uint32_t)(it.q_token + token)), (int)p.shared);
     }
-    template <int DP>
-    __device__ void finish(const BigItem& it, int t, int row, int token, bool mine, bool any, uint32_t to, float m,
-                           float l, float shift) const {
-        if (!any) return;
+    __device__ void result(const BigItem& it, int row, int token, float m, float l, float shift, uint8_t*& dst,
+                           float& factor) const {
         const size_t rows = (size_t)p.batch * p.group;
         const size_t at = ((size_t)it.slot * p.kv_heads + it.head) * rows + (size_t)(it.q_token + token) * p.group + row % p.group;
-        if (mine) *reinterpret_cast<float2*>(p.pm + at * 2) = make_float2(m, l);
-#pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(to + c, o);
-            ptx::tmem_ld_wait();
-            ptx::pin32(o);
-            if (mine) store32(reinterpret_cast<uint8_t*>(p.po + at * p.dim), c, p.dim, ANE_DTYPE_F32, o, 1.0f);
-        }
+        *reinterpret_cast<float2*>(p.pm + at * 2) = make_float2(m, l);
+        dst = reinterpret_cast<uint8_t*>(p.po + at * p.dim);
+        factor = l == 0.0f ? 0.0f : 1.0f;
     }
+    __device__ uint32_t dim() const { return p.dim; }
+    __device__ uint32_t out_dtype() const { return ANE_DTYPE_F32; }
 };
 
 template <typename T, int DP>
@@ -695,8 +686,7 @@ int launch(const CUtensorMap (&map)[3], const Params& p, uint32_t pairs, cudaStr
     if (p.big_splits) {
         if ((rc = set_max_dynamic_smem(prefix_kernel<T, DP>, (int)big_smem_bytes<DP>(), done_big))) return rc;
         const uint64_t items = (uint64_t)p.big_splits * p.kv_heads * pairs;
-        uint64_t blocks = items < (uint64_t)num_sms() ? items : (uint64_t)num_sms();
-        if (blocks * kMaxItems < items) blocks = ceil_div(items, kMaxItems);
+        const uint64_t blocks = items < (uint64_t)num_sms() ? items : (uint64_t)num_sms();
         if ((rc = launch_pdl(prefix_kernel<T, DP>, dim3((uint32_t)blocks), dim3(kBigThreads), big_smem_bytes<DP>(), s,
                              map[0], map[1], map[2], p, pairs)))
             return rc;

@@ -27,7 +27,8 @@ struct Seq {
 // Counts that point outside the buffers are cut to them: nothing is read or
 // written out of range whatever cu_q and cu_k hold.
 __device__ __forceinline__ Seq sequence(const Params& p, uint32_t s) {
-    Seq r;
+    Seq r{0, 0, 0, 0};
+    if (s >= p.n_seq) return r;
     r.q0 = p.cu_q[s];
     r.k0 = p.cu_k[s];
     r.lq = min(p.cu_q[s + 1], (int)p.total_q) - r.q0;
@@ -48,15 +49,17 @@ __device__ __forceinline__ int items_from_level(const Seq& s, int L, int w) {
 
 struct PromptJob {
     const Params& p;
+    Seq mine;  // of warp 11: sequence `lane`, the first 32 of them kept
 
+    __device__ Seq get(uint32_t s) const { return s < 32 ? mine : sequence(p, s); }
     // Item number `o` in order of falling key tiles.  A whole warp.
-    __device__ BigItem find(int o) const {
+    __device__ BigItem find(int o) {
         const int lane = threadIdx.x & 31, w = 2 * (int)p.tile_tokens;
+        if (mine.lq < 0) mine = sequence(p, lane);
         auto count = [&](int L) {
             int c = 0;
-            for (uint32_t s = lane; s < p.n_seq; s += 32) c += items_from_level(sequence(p, s), L, w);
-            for (int d = 16; d; d >>= 1) c += __shfl_xor_sync(0xffffffffu, c, d);
-            return c;
+            for (uint32_t s = lane; s < p.n_seq; s += 32) c += items_from_level(get(s), L, w);
+            return (int)__reduce_add_sync(0xffffffffu, c);
         };
         BigItem it{};
         it.head = -1;
@@ -68,9 +71,7 @@ struct PromptJob {
         }
         int r = o - count(hi);
         for (uint32_t s0 = 0; s0 < p.n_seq; s0 += 32) {
-            const uint32_t s = s0 + lane;
-            Seq q{0, 0, 0, 0};
-            if (s < p.n_seq) q = sequence(p, s);
+            const Seq q = get(s0 + lane);
             const int a = items_from_level(q, lo, w), b = items_from_level(q, lo + 1, w);
             int sum = a - b;
             for (int d = 1; d < 32; d <<= 1) {
@@ -100,55 +101,36 @@ struct PromptJob {
         }
         return it;
     }
-    __device__ void items(BigItem* list) const {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        bool more = true;
-        for (int i = warp; i < kMaxItems; i += kBigThreads / 32) {
-            const uint32_t w = i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-            BigItem it{};
-            it.head = -1;
-            if (more) it = find((int)(w / p.kv_heads));
-            if (it.head >= 0) it.head = (int)(w % p.kv_heads);
-            else more = false;
-            if (lane == 0) list[i] = it;
-        }
+    __device__ BigItem item(int i) {
+        const uint64_t w = (uint64_t)i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        BigItem it{};
+        it.head = -1;
+        if (w < 0x7fffffffu) it = find((int)(w / p.kv_heads));
+        if (it.head >= 0) it.head = (int)(w % p.kv_heads);
+        return it;
     }
     __device__ int box_keys() const { return kBigKeys; }
     __device__ int2 coord(const BigItem& it, int key) const { return make_int2(it.k0 + key, 0); }
     __device__ int visible(const BigItem& it, int token) const { return max(0, min(it.lk, it.see + token + 1)); }
 
-    template <int DP>
-    __device__ void finish(const BigItem& it, int t, int row, int token, bool mine, bool any, uint32_t to, float m,
-                           float l, float shift) const {
+    __device__ void result(const BigItem& it, int row, int token, float m, float l, float shift, uint8_t*& dst,
+                           float& factor) const {
         const uint32_t head = it.head * p.group + row % p.group;
         const size_t q = (size_t)it.q_token + token;
-        uint8_t* dst = static_cast<uint8_t*>(p.out.data) +
-                       (q * p.out.token_stride + head * p.out.head_stride) * (p.out_dtype == ANE_DTYPE_F32 ? 4 : 2);
-        const bool empty = l == 0.0f;
-        const float inv = empty ? 0.0f : 1.0f / l;
-#pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            if (any) {
-                ptx::tmem_ld_32x32b_x32(to + c, o);
-                ptx::tmem_ld_wait();
-                ptx::pin32(o);
-            }
-            if (empty || !any) {  // 0, whatever the accumulator holds
-#pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = 0;
-            }
-            if (mine) store32(dst, c, p.dim, p.out_dtype, o, inv);
-        }
-        if (mine && p.lse) p.lse[q * p.heads + head] = empty ? kNegInf : (m + log2f(l) - shift) * kLn2;
+        dst = static_cast<uint8_t*>(p.out.data) +
+              (q * p.out.token_stride + head * p.out.head_stride) * (p.out_dtype == ANE_DTYPE_F32 ? 4 : 2);
+        factor = l == 0.0f ? 0.0f : 1.0f / l;
+        if (p.lse) p.lse[q * p.heads + head] = l == 0.0f ? kNegInf : (m + log2f(l) - shift) * kLn2;
     }
+    __device__ uint32_t dim() const { return p.dim; }
+    __device__ uint32_t out_dtype() const { return p.out_dtype; }
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBigThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const Params p) {
-    PromptJob job{p};
+    PromptJob job{p, {0, 0, -1, 0}};
     big_attention<T, DP>(&map_q, &map_k, &map_v, p.group, p.scale2, p.err, job);
 }
 
@@ -159,8 +141,7 @@ int launch(const CUtensorMap (&map)[3], const Params& p, cudaStream_t s) {
     if (rc) return rc;
     // the lengths are on the device: as many items as total_q tokens in n_seq pieces can make
     const uint64_t items = (uint64_t)(p.total_q / (2 * p.tile_tokens) + p.n_seq) * p.kv_heads;
-    uint64_t blocks = items < (uint64_t)num_sms() ? items : (uint64_t)num_sms();
-    if (blocks * kMaxItems < items) blocks = ceil_div(items, kMaxItems);
+    const uint64_t blocks = items < (uint64_t)num_sms() ? items : (uint64_t)num_sms();
     return launch_pdl(prompt_kernel<T, DP>, dim3((uint32_t)blocks), dim3(kBigThreads), big_smem_bytes<DP>(), s, map[0],
                       map[1], map[2], p);
 }

@@ -14,9 +14,15 @@
 // stand and cancel against the row sum, which is kept in fp32.  F16 weights are
 // stored 2^6 times larger (2^14 at most), as attn_core.cuh explains.
 //
+// What bounds it: per tile of 128 x 128 scores and head dim 128 the tensor cores
+// take 1024 cycles (both products), the 16384 exponentials 1024 cycles of the
+// special-function unit, and each tile's products wait for its exponentials.  So
+// three of eight exponentials are a polynomial on the FMA units instead, and the
+// first half of P is handed over while the second is computed.
+//
 // Warps (384 threads): 0-3 and 4-7 softmax of tile 0 and 1; 8 loads (TMA);
 // 9 issues the MMAs and owns TMEM; 10 clears the rows of V that lie past the
-// last key (a weight of 0 does not silence a NaN there); 11 idles.
+// last key (a weight of 0 does not silence a NaN there); 11 finds the items.
 // Registers: 384 x 168 at launch; 256 x 208 + 128 x 88 after the split, the same
 // 64,512.
 #pragma once
@@ -28,8 +34,9 @@ namespace attn {
 constexpr int kBigThreads = 384;
 constexpr int kBigRows = 128;    // rows of a query tile
 constexpr int kBigKeys = 128;    // keys of a key/value tile
+constexpr int kPolyOf8 = 3;      // exponentials of eight that are polynomials
 constexpr float kSlack = 8.0f;   // log2 of how far weights may pass 1
-constexpr int kMaxItems = 32;    // items per block
+constexpr int kItemRing = 4;     // items announced ahead
 
 struct BigItem {
     int q_token;     // first query token (a row of q); tokens of the item: `tokens`
@@ -45,14 +52,16 @@ struct BigItem {
 
 template <int DP>
 struct BigSmem {
-    static constexpr int kStages = DP == 128 ? 5 : 10;
+    static constexpr int kStages = DP == 128 ? 4 : 8;
     static constexpr int kTileBytes = 128 * DP * 2;
     uint8_t q[2][kTileBytes];
     uint8_t kv[kStages][kTileBytes];
+    uint8_t out[8][32 * 128];  // per softmax warp: 128 bytes of 32 result rows
     uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages], tail_full[kStages];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
+    uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint32_t tmem;
-    BigItem items[kMaxItems];
+    BigItem items[kItemRing];
 };
 template <int DP>
 constexpr size_t big_smem_bytes() {
@@ -72,12 +81,105 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
+__device__ __forceinline__ float2 add_down2(float2 a, float2 b) {  // rounded towards -infinity
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\t"
+        "mov.b64 rb, {%4, %5};\n\t"
+        "add.rm.f32x2 rd, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// 2^x of two values below 128 on the FMA units: x = n + f with n = floor(x), 2^f
+// a polynomial on [0, 1) and n added to its exponent.  The polynomial is 1 at
+// f = 0 and minimises the largest relative error, 2.9e-6 (a least-squares fit
+// reweighted towards the worst points); values from -127 down give exactly 0.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    x.x = fmaxf(x.x, -127.0f);
+    x.y = fmaxf(x.y, -127.0f);
+    const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: n in the low bits
+    const float2 t = add_down2(x, big);
+    const float2 n = ptx::fadd2(t, make_float2(-12582912.0f, -12582912.0f));
+    const float2 f = ptx::ffma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 p = ptx::ffma2(f, make_float2(1.342668553e-02f, 1.342668553e-02f), make_float2(5.224247220e-02f, 5.224247220e-02f));
+    p = ptx::ffma2(p, f, make_float2(2.412802057e-01f, 2.412802057e-01f));
+    p = ptx::ffma2(p, f, make_float2(6.930448448e-01f, 6.930448448e-01f));
+    p = ptx::ffma2(p, f, make_float2(1.0f, 1.0f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// One warp: the DP accumulator columns of its 32 rows (TMEM address `to`), times
+// factor, to each row's dst (NULL: no such row), rounded to out_dtype.  128 bytes
+// of every row at a time go through shared memory, so that a store instruction
+// writes four rows' whole lines (a row per lane would touch 32 lines).
+// any: false if there is no accumulator (the rows are 0).
+template <int DP>
+__device__ __forceinline__ void store_rows(uint8_t* stage, uint8_t* dst, float factor, bool any, uint32_t to,
+                                           uint32_t dim, uint32_t out_dtype) {
+    const int lane = threadIdx.x & 31;
+    const int cols = out_dtype == ANE_DTYPE_F32 ? 32 : 64;
+    const uint32_t row_bytes = dim * (out_dtype == ANE_DTYPE_F32 ? 4 : 2);
+#pragma unroll 1
+    for (int c = 0; c < DP; c += cols) {
+#pragma unroll 1
+        for (int half = 0; half < cols / 32; half++) {
+            uint32_t o[32];
+            if (any) {
+                ptx::tmem_ld_32x32b_x32(to + c + half * 32, o);
+                ptx::tmem_ld_wait();
+                ptx::pin32(o);
+            }
+            const bool zero = !any || factor == 0.0f;  // whatever the accumulator holds
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = zero ? 0u : __float_as_uint(__uint_as_float(o[i]) * factor);
+            auto put = [&](int chunk, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+                *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = make_uint4(a, b, d, e);
+            };
+            if (out_dtype == ANE_DTYPE_F32) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) put(i, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float x = __uint_as_float(o[8 * i + 2 * k]), y = __uint_as_float(o[8 * i + 2 * k + 1]);
+                        w[k] = out_dtype == ANE_DTYPE_F16 ? Type<__half>::pack(x, y) : Type<__nv_bfloat16>::pack(x, y);
+                    }
+                    put(half * 4 + i, w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        __syncwarp();
+        const uint32_t at = (uint32_t)(c / cols) * 128 + (lane & 7) * 16;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = i * 4 + (lane >> 3);
+            uint8_t* d = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            if (d && at < row_bytes) *reinterpret_cast<uint4*>(d + at) = v;
+        }
+        __syncwarp();
+    }
+}
+
 // The kernel's frame.  Job supplies:
-//   items(sm.items)             all warps: this block's items, ended by head -1
+//   item(i)                     item i of this block (a whole warp; head -1: no more)
 //   box_keys()                  keys per TMA box (a multiple of 8 that divides 128)
 //   coord(item, key)            {token, page} coordinates of the box that starts at a key
 //   visible(item, token)        keys that query token `token` of the item sees
-//   finish(item, t, token, row, tmem_o, m, l)   one thread per row
+//   result(item, row, token, m, l, shift, dst, factor)  where a row's result goes, what it is
+//                               multiplied by (0: it is 0), its statistics written
+//   out_dtype(), dim()
 template <typename T, int DP, class Job>
 __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CUtensorMap* map_k,
                                               const CUtensorMap* map_v, uint32_t group, float scale2, int* err,
@@ -89,7 +191,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
     constexpr int kBoxBytes = 128 * 128;
     constexpr float kShift = Type<T>::kShift;  // with kSlack: F16 weights stay below 2^14
     constexpr bool kBf16 = Type<T>::kShift == 0.0f;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int tile_tokens = kBigRows / (int)group;
 
     if (threadIdx.x == 0) {
@@ -102,8 +204,13 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
         }
         for (int t = 0; t < 2; t++) {
             ptx::mbar_init(&sm.s_full[t], 1);
+            ptx::mbar_init(&sm.p_half[t], 4);
             ptx::mbar_init(&sm.p_full[t], 4);
             ptx::mbar_init(&sm.o_full[t], 1);
+        }
+        for (int i = 0; i < kItemRing; i++) {
+            ptx::mbar_init(&sm.item_full[i], 1);
+            ptx::mbar_init(&sm.item_empty[i], 11);  // 8 softmax warps, loads, MMAs, V rows
         }
         ptx::fence_mbarrier_init();
         ptx::prefetch_tmap(map_q);
@@ -118,11 +225,19 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
     // work before this one (attn_decode.cu)
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    job.items(sm.items);
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = sm.tmem;  // columns: S0 0, S1 128, O0 256, O1 384
+    // item i, for a whole warp; false: no more, or gave up
+    auto take = [&](int i, BigItem& it) {
+        const int e = i % kItemRing;
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(&sm.item_full[e], (i / kItemRing) & 1, err))) return false;
+        it = sm.items[e];
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sm.item_empty[e]);
+        return __all_sync(0xffffffffu, it.head >= 0) != 0;
+    };
 
     if (warp >= 8) {
         ptx::regs_dec<88>();
@@ -134,9 +249,8 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
             const uint32_t dst0 = lane % kBoxes * kBoxBytes + key0 * 128;
             uint32_t n = 0, used = 0;
             bool ok = true;
-            for (int i = 0; i < kMaxItems && ok; i++) {
-                const BigItem it = sm.items[i];
-                if (it.head < 0) break;
+            BigItem it;
+            for (int i = 0; ok && take(i, it); i++) {
                 const int end = max(it.end[0], it.end[1]);
                 if (end <= it.begin) continue;
                 int2 at = lane < boxes ? job.coord(it, it.begin * kBigKeys + key0) : make_int2(0, 0);
@@ -166,78 +280,94 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                     at = next;
                 }
             }
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 9) {
             // ----------------------------------------------------------- MMAs
+            // The whole warp goes through the loop on values that the compiler
+            // can see are the same in all lanes, and one elected lane issues:
+            // descriptors then stay in uniform registers (a lane on its own
+            // moves them there for every MMA, which took longer than the MMA).
             constexpr uint32_t idesc_s = ptx::idesc_f16(kBigRows, kBigKeys, kBf16);
             constexpr uint32_t idesc_o = ptx::idesc_f16(kBigRows, DP, kBf16) | ptx::kIdescBMnMajor;
-            uint32_t n = 0, used = 0, pc[2] = {0, 0};
+            const bool lead = ptx::elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t q_base = ptx::smem_u32(sm.q[0]), kv_base = ptx::smem_u32(sm.kv[0]);
+            uint32_t n = 0, used = 0, pc0 = 0, pc1 = 0;
             bool ok = true;
-            auto full = [&](uint32_t m) {
-                ok = ptx::mbar_wait(&sm.kv_full[m % S::kStages], (m / S::kStages) & 1, err);
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, err));
                 if (ok) ptx::tc_fence_after();
                 return ok;
             };
+            auto full = [&](uint32_t m) { return wait(&sm.kv_full[m % S::kStages], (m / S::kStages) & 1); };
+            auto commit = [&](uint64_t* bar) {
+                if (lead) ptx::umma_commit(bar);
+                __syncwarp();
+            };
             auto qk = [&](int t, uint32_t m) {
-                const uint32_t a = ptx::smem_u32(sm.q[t]), b = ptx::smem_u32(sm.kv[m % S::kStages]);
+                const uint32_t a = q_base + t * S::kTileBytes, b = kv_base + (m % S::kStages) * S::kTileBytes;
+                if (lead) {
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; kk++)
-                    ptx::umma_f16(tmem + t * 128, desc_k(a, kk), desc_k(b, kk), idesc_s, kk != 0);
-                ptx::umma_commit(&sm.s_full[t]);
+                    for (int kk = 0; kk < DP / 16; kk++)
+                        ptx::umma_f16(tm + t * 128, desc_k(a, kk), desc_k(b, kk), idesc_s, kk != 0);
+                    ptx::umma_commit(&sm.s_full[t]);
+                }
+                __syncwarp();
             };
-            auto pv = [&](int t, uint32_t m, bool add) {
-                const uint32_t b = ptx::smem_u32(sm.kv[m % S::kStages]);
+            auto pv = [&](int t, uint32_t m, bool add, int half) {  // 64 keys
+                const uint32_t b = kv_base + (m % S::kStages) * S::kTileBytes;
+                if (lead) {
 #pragma unroll
-                for (int kk = 0; kk < kBigKeys / 16; kk++)
-                    ptx::umma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
-                                     ptx::sdesc_mn(b + kk * 2048, 128, kBoxBytes), idesc_o, add || kk != 0);
+                    for (int kk = 0; kk < 4; kk++)
+                        ptx::umma_f16_ta(tm + 256 + t * 128, tm + t * 128 + (half * 4 + kk) * 8,
+                                         ptx::sdesc_mn(b + (half * 4 + kk) * 2048, 128, kBoxBytes), idesc_o, add || kk != 0);
+                }
+                __syncwarp();
             };
-            for (int i = 0; i < kMaxItems && ok; i++) {
-                const BigItem it = sm.items[i];
-                if (it.head < 0) break;
-                const int end = max(it.end[0], it.end[1]);
-                if (end <= it.begin) continue;
-                if (!ptx::mbar_wait(&sm.q_full, used & 1, err)) break;
+            BigItem it;
+            for (int i = 0; ok && take(i, it); i++) {
+                const int begin = __shfl_sync(0xffffffffu, it.begin, 0);
+                const int end0 = __shfl_sync(0xffffffffu, it.end[0], 0), end1 = __shfl_sync(0xffffffffu, it.end[1], 0);
+                const int end = max(end0, end1);
+                if (end <= begin) continue;
+                if (!wait(&sm.q_full, used & 1) || !full(n)) break;
                 used++;
-                if (!full(n)) break;
-                for (int t = 0; t < 2; t++)
-                    if (it.begin < it.end[t]) qk(t, n);
-                ptx::umma_commit(&sm.kv_empty[n % S::kStages]);
+                if (begin < end0) qk(0, n);
+                if (begin < end1) qk(1, n);
+                commit(&sm.kv_empty[n % S::kStages]);
                 n++;
-                if (end == it.begin + 1) ptx::umma_commit(&sm.q_empty);
-                for (int j = it.begin; j < end && ok; j++) {
+                if (end == begin + 1) commit(&sm.q_empty);
+                for (int j = begin; j < end; j++) {
                     const uint32_t nv = n;
                     const bool next = j + 1 < end;
-                    if (!full(nv)) break;
-                    bool have_k = false;
-                    for (int t = 0; t < 2 && ok; t++) {
-                        if (j >= it.end[t]) continue;
-                        if (!(ok = ptx::mbar_wait(&sm.p_full[t], pc[t] & 1, err))) break;
-                        pc[t]++;
-                        ptx::tc_fence_after();
-                        pv(t, nv, j > it.begin);
-                        if (j == it.end[t] - 1) ptx::umma_commit(&sm.o_full[t]);
-                        if (j + 1 < it.end[t]) {
-                            if (!have_k && !full(nv + 1)) break;
-                            have_k = true;
-                            qk(t, nv + 1);
-                        }
+                    if (!full(nv) || (next && !full(nv + 1))) break;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const int et = t ? end1 : end0;
+                        if (j >= et) continue;
+                        uint32_t& pc = t ? pc1 : pc0;
+                        if (!wait(&sm.p_half[t], pc & 1)) break;
+                        pv(t, nv, j > begin, 0);
+                        if (!wait(&sm.p_full[t], pc & 1)) break;
+                        pc++;
+                        pv(t, nv, true, 1);
+                        if (j == et - 1) commit(&sm.o_full[t]);
+                        else qk(t, nv + 1);
                     }
                     if (!ok) break;
-                    ptx::umma_commit(&sm.kv_empty[nv % S::kStages]);
+                    commit(&sm.kv_empty[nv % S::kStages]);
                     n = nv + 1;
                     if (next) {
-                        ptx::umma_commit(&sm.kv_empty[n % S::kStages]);
+                        commit(&sm.kv_empty[n % S::kStages]);
                         n++;
-                        if (j + 2 == end) ptx::umma_commit(&sm.q_empty);
+                        if (j + 2 == end) commit(&sm.q_empty);
                     }
                 }
             }
         } else if (warp == 10) {
             // -------------------------------------------- rows of V past the end
             uint32_t n = 0, phase = 0;  // phase: bit per stage
-            for (int i = 0; i < kMaxItems; i++) {
-                const BigItem it = sm.items[i];
-                if (it.head < 0) break;
+            BigItem it;
+            for (int i = 0; take(i, it); i++) {
                 const int end = max(it.end[0], it.end[1]);
                 if (end <= it.begin) continue;
                 n += 2 * (uint32_t)(end - it.begin);  // V of the last tile is number n - 1
@@ -254,6 +384,18 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&sm.kv_full[st]);
             }
+        } else if (warp == 11) {
+            // ---------------------------------------------------------- items
+            for (int i = 0;; i++) {
+                const BigItem it = job.item(i);
+                const int e = i % kItemRing;
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait(&sm.item_empty[e], ((i / kItemRing) & 1) ^ 1, err))) break;
+                if (lane == 0) {
+                    sm.items[e] = it;
+                    ptx::mbar_arrive(&sm.item_full[e]);
+                }
+                if (it.head < 0) break;
+            }
         }
     } else {
         // ------------------------------------------------------------- softmax
@@ -266,9 +408,8 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
         const bool real = row < tile_tokens * (int)group;
         uint32_t sc = 0, oc = 0;
         bool ok = true;
-        for (int i = 0; i < kMaxItems && ok; i++) {
-            const BigItem it = sm.items[i];
-            if (it.head < 0) break;
+        BigItem it;
+        for (int i = 0; ok && take(i, it); i++) {
             const bool mine = real && token < it.tokens;
             const int vis = mine ? job.visible(it, token) : 0;
             float m = kNegInf, l = 0.0f;
@@ -296,9 +437,14 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 for (int c = 0; c < 4; c++) {
                     mx[c] = __uint_as_float(s[c][0]);
 #pragma unroll
-                    for (int x = 1; x < 32; x++) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][x]));
+                    for (int x = 1; x < 31; x += 2)
+                        mx[c] = max3_nan(mx[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                mx[0] = max3_nan(mx[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
+                mx[1] = max3_nan(mx[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
+                const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale2;
+                // a NaN or an infinite score makes the whole row NaN
+                if (!(top < INFINITY)) l = NAN;
                 if (__any_sync(0xffffffffu, top > m + kSlack)) {
                     const float mn = fmaxf(m, top), base = mn == kNegInf ? 0.0f : mn;
                     const float c = exp2_fast(m - base);
@@ -327,18 +473,22 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                     for (int x = 0; x < 32; x++) {
                         const uint32_t* v = &s[2 * h + (x >> 4)][2 * (x & 15)];
                         float2 e = ptx::ffma2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), sc2, off2);
-                        e.x = exp2_fast(e.x);
-                        e.y = exp2_fast(e.y);
+                        if (x % 8 < kPolyOf8) {
+                            e = exp2_poly(e);
+                        } else {
+                            e.x = exp2_fast(e.x);
+                            e.y = exp2_fast(e.y);
+                        }
                         sum[x & 1] = ptx::fadd2(sum[x & 1], e);
                         w[x] = Type<T>::pack(e.x, e.y);
                     }
                     ptx::tmem_st_32x32b_x32(ts + h * 32, w);
+                    ptx::tmem_st_wait();
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(h ? &sm.p_full[t] : &sm.p_half[t]);
                 }
                 l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
-                ptx::tmem_st_wait();
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&sm.p_full[t]);
             }
             if (!ok) break;
             if (it.begin < it.end[t]) {
@@ -347,8 +497,10 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 oc++;
                 ptx::tc_fence_after();
             }
-            // rows without a tile skip TMEM; the whole warp takes part in the reads
-            job.template finish<DP>(it, t, row, token, mine, it.begin < it.end[t], to, m, l, kShift);
+            uint8_t* dst = nullptr;
+            float factor = 0.0f;
+            if (mine) job.result(it, row, token, m, l, kShift, dst, factor);
+            store_rows<DP>(sm.out[warp], dst, factor, it.begin < it.end[t], to, job.dim(), job.out_dtype());
             ptx::tc_fence_before();
         }
     }
@@ -358,31 +510,6 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
     if (warp == 9) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 512);
-    }
-}
-
-// Columns c .. c + 31 of a result row (16-byte aligned), times inv.
-__device__ __forceinline__ void store32(uint8_t* row, uint32_t c, uint32_t dim, uint32_t out_dtype,
-                                        const uint32_t (&o)[32], float inv) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        if (c + i >= dim) continue;
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = __uint_as_float(o[i + j]) * inv;
-        if (out_dtype == ANE_DTYPE_F32) {
-            float4* d = reinterpret_cast<float4*>(row + (size_t)(c + i) * 4);
-            d[0] = make_float4(f[0], f[1], f[2], f[3]);
-            d[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else if (out_dtype == ANE_DTYPE_F16) {
-            *reinterpret_cast<uint4*>(row + (size_t)(c + i) * 2) =
-                make_uint4(Type<__half>::pack(f[0], f[1]), Type<__half>::pack(f[2], f[3]),
-                           Type<__half>::pack(f[4], f[5]), Type<__half>::pack(f[6], f[7]));
-        } else {
-            *reinterpret_cast<uint4*>(row + (size_t)(c + i) * 2) =
-                make_uint4(Type<__nv_bfloat16>::pack(f[0], f[1]), Type<__nv_bfloat16>::pack(f[2], f[3]),
-                           Type<__nv_bfloat16>::pack(f[4], f[5]), Type<__nv_bfloat16>::pack(f[6], f[7]));
-        }
     }
 }
 
