@@ -17,8 +17,10 @@
 // What bounds it: per tile of 128 x 128 scores and head dim 128 the tensor cores
 // take 1024 cycles (both products), the 16384 exponentials 1024 cycles of the
 // special-function unit, and each tile's products wait for its exponentials.  So
-// three of eight exponentials are a polynomial on the FMA units instead, and the
-// first half of P is handed over while the second is computed.
+// P is handed over in parts while the rest is computed, and a tile's first
+// weights do not wait for its maximum.  (Some of the exponentials as a polynomial
+// on the FMA units was slower, 16384 tokens: 0, 2, 3, 4 of eight 1613, 1791, 1790,
+// 1899 us.)
 //
 // Warps (384 threads): 0-3 and 4-7 softmax of tile 0 and 1; 8 loads (TMA);
 // 9 issues the MMAs and owns TMEM; 10 clears the rows of V that lie past the
@@ -34,7 +36,6 @@ namespace attn {
 constexpr int kBigThreads = 384;
 constexpr int kBigRows = 128;    // rows of a query tile
 constexpr int kBigKeys = 128;    // keys of a key/value tile
-constexpr int kPolyOf8 = 3;      // exponentials of eight that are polynomials
 constexpr float kSlack = 8.0f;   // log2 of how far weights may pass 1
 constexpr int kItemRing = 4;     // items announced ahead
 
@@ -58,7 +59,7 @@ struct BigSmem {
     uint8_t kv[kStages][kTileBytes];
     uint8_t out[8][32 * 128];  // per softmax warp: 128 bytes of 32 result rows
     uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages], tail_full[kStages];
-    uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_part[3][2], o_full[2];  // P: 64, 32 and 32 keys
     uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint32_t tmem;
     BigItem items[kItemRing];
@@ -81,38 +82,9 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
-__device__ __forceinline__ float2 add_down2(float2 a, float2 b) {  // rounded towards -infinity
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-        "mov.b64 ra, {%2, %3};\n\t"
-        "mov.b64 rb, {%4, %5};\n\t"
-        "add.rm.f32x2 rd, ra, rb;\n\t"
-        "mov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-// 2^x of two values below 128 on the FMA units: x = n + f with n = floor(x), 2^f
-// a polynomial on [0, 1) and n added to its exponent.  The polynomial is 1 at
-// f = 0 and minimises the largest relative error, 2.9e-6 (a least-squares fit
-// reweighted towards the worst points); values from -127 down give exactly 0.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    x.x = fmaxf(x.x, -127.0f);
-    x.y = fmaxf(x.y, -127.0f);
-    const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: n in the low bits
-    const float2 t = add_down2(x, big);
-    const float2 n = ptx::fadd2(t, make_float2(-12582912.0f, -12582912.0f));
-    const float2 f = ptx::ffma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 p = ptx::ffma2(f, make_float2(1.342668553e-02f, 1.342668553e-02f), make_float2(5.224247220e-02f, 5.224247220e-02f));
-    p = ptx::ffma2(p, f, make_float2(2.412802057e-01f, 2.412802057e-01f));
-    p = ptx::ffma2(p, f, make_float2(6.930448448e-01f, 6.930448448e-01f));
-    p = ptx::ffma2(p, f, make_float2(1.0f, 1.0f));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -204,8 +176,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
         }
         for (int t = 0; t < 2; t++) {
             ptx::mbar_init(&sm.s_full[t], 1);
-            ptx::mbar_init(&sm.p_half[t], 4);
-            ptx::mbar_init(&sm.p_full[t], 4);
+            for (int x = 0; x < 3; x++) ptx::mbar_init(&sm.p_part[x][t], 4);
             ptx::mbar_init(&sm.o_full[t], 1);
         }
         for (int i = 0; i < kItemRing; i++) {
@@ -313,13 +284,13 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 }
                 __syncwarp();
             };
-            auto pv = [&](int t, uint32_t m, bool add, int half) {  // 64 keys
+            auto pv = [&](int t, uint32_t m, bool add, int first, int last) {  // 16-key steps
                 const uint32_t b = kv_base + (m % S::kStages) * S::kTileBytes;
                 if (lead) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        ptx::umma_f16_ta(tm + 256 + t * 128, tm + t * 128 + (half * 4 + kk) * 8,
-                                         ptx::sdesc_mn(b + (half * 4 + kk) * 2048, 128, kBoxBytes), idesc_o, add || kk != 0);
+                    for (int kk = first; kk < last; kk++)
+                        ptx::umma_f16_ta(tm + 256 + t * 128, tm + t * 128 + kk * 8,
+                                         ptx::sdesc_mn(b + kk * 2048, 128, kBoxBytes), idesc_o, add || kk != 0);
                 }
                 __syncwarp();
             };
@@ -345,11 +316,13 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                         const int et = t ? end1 : end0;
                         if (j >= et) continue;
                         uint32_t& pc = t ? pc1 : pc0;
-                        if (!wait(&sm.p_half[t], pc & 1)) break;
-                        pv(t, nv, j > begin, 0);
-                        if (!wait(&sm.p_full[t], pc & 1)) break;
+                        if (!wait(&sm.p_part[0][t], pc & 1)) break;
+                        pv(t, nv, j > begin, 0, 4);
+                        if (!wait(&sm.p_part[1][t], pc & 1)) break;
+                        pv(t, nv, true, 4, 6);
+                        if (!wait(&sm.p_part[2][t], pc & 1)) break;
                         pc++;
-                        pv(t, nv, true, 1);
+                        pv(t, nv, true, 6, 8);
                         if (j == et - 1) commit(&sm.o_full[t]);
                         else qk(t, nv + 1);
                     }
@@ -418,34 +391,37 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 if (!ok) break;
                 sc++;
                 ptx::tc_fence_after();
-                uint32_t s[4][32];
+                uint32_t s[4][32], w[16];
+                float2 sum[2];
+                const float2 sc2 = make_float2(scale2, scale2);
+                // weights of keys 32 c .. 32 c + 31 of the tile
+                auto weights = [&](int c) {
+                    const float off = kShift - (m == kNegInf ? 0.0f : m);
+                    const float2 off2 = make_float2(off, off);
 #pragma unroll
-                for (int c = 0; c < 4; c++) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
-                ptx::tmem_ld_wait();
+                    for (int x = 0; x < 16; x++) {
+                        float2 e = ptx::ffma2(make_float2(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), sc2, off2);
+                        e.x = exp2_fast(e.x);
+                        e.y = exp2_fast(e.y);
+                        sum[x & 1] = c == 0 && x < 2 ? e : ptx::fadd2(sum[x & 1], e);
+                        w[x] = Type<T>::pack(e.x, e.y);
+                    }
+                };
+                auto largest = [&] {
+                    float mx[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) ptx::pin32(s[c]);
-                const int rest = vis - j * kBigKeys;  // keys of this tile that the row sees
-                if (__any_sync(0xffffffffu, rest < kBigKeys)) {
-                    // selected, not added: a hidden score may be anything, NaN included
+                    for (int c = 0; c < 4; c++) {
+                        mx[c] = __uint_as_float(s[c][0]);
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int x = 0; x < 32; x++) s[c][x] = c * 32 + x < rest ? s[c][x] : 0xff800000u;
-                }
-                float mx[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-                    for (int x = 1; x < 31; x += 2)
-                        mx[c] = max3_nan(mx[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
-                }
-                mx[0] = max3_nan(mx[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
-                mx[1] = max3_nan(mx[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
-                const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale2;
-                // a NaN or an infinite score makes the whole row NaN
-                if (!(top < INFINITY)) l = NAN;
-                if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                        for (int x = 1; x < 31; x += 2)
+                            mx[c] = max3(mx[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
+                    }
+                    mx[0] = max3(mx[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
+                    mx[1] = max3(mx[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
+                    return max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale2;
+                };
+                // moves the rows' references to their maxima so far
+                auto raise = [&](float top) {
                     const float mn = fmaxf(m, top), base = mn == kNegInf ? 0.0f : mn;
                     const float c = exp2_fast(m - base);
                     if (j > it.begin) {
@@ -462,32 +438,59 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                     }
                     l *= c;
                     m = mn;
-                }
-                const float off = kShift - (m == kNegInf ? 0.0f : m);
-                const float2 sc2 = make_float2(scale2, scale2), off2 = make_float2(off, off);
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int x = 0; x < 32; x++) {
-                        const uint32_t* v = &s[2 * h + (x >> 4)][2 * (x & 15)];
-                        float2 e = ptx::ffma2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), sc2, off2);
-                        if (x % 8 < kPolyOf8) {
-                            e = exp2_poly(e);
-                        } else {
-                            e.x = exp2_fast(e.x);
-                            e.y = exp2_fast(e.y);
-                        }
-                        sum[x & 1] = ptx::fadd2(sum[x & 1], e);
-                        w[x] = Type<T>::pack(e.x, e.y);
-                    }
-                    ptx::tmem_st_32x32b_x32(ts + h * 32, w);
+                };
+                auto arrive = [&](int part) {
                     ptx::tmem_st_wait();
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(h ? &sm.p_full[t] : &sm.p_half[t]);
+                    if (lane == 0) ptx::mbar_arrive(&sm.p_part[part][t]);
+                };
+                const int rest = vis - j * kBigKeys;  // keys of this tile that the row sees
+                float top;
+                if (j > it.begin && __all_sync(0xffffffffu, rest >= kBigKeys)) {
+                    // The reference of the tiles before will do for this one too,
+                    // nearly always: its first weights are under way before the
+                    // tile's maximum is known.
+                    ptx::tmem_ld_32x32b_x32(ts, s[0]);
+                    ptx::tmem_ld_wait();
+                    ptx::pin32(s[0]);
+#pragma unroll
+                    for (int c = 1; c < 4; c++) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
+                    weights(0);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int c = 1; c < 4; c++) ptx::pin32(s[c]);
+                    top = largest();
+                    if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                        raise(top);
+                        weights(0);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 4; c++) ptx::pin32(s[c]);
+                    // selected, not added: a hidden score may be anything, NaN included
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int x = 0; x < 32; x++) s[c][x] = c * 32 + x < rest ? s[c][x] : 0xff800000u;
+                    top = largest();
+                    if (__any_sync(0xffffffffu, top > m + kSlack)) raise(top);
+                    weights(0);
                 }
+                // P goes out while the next keys' weights are computed
+                ptx::tmem_st_32x32b_x16(ts, w);
+                weights(1);
+                ptx::tmem_st_32x32b_x16(ts + 16, w);
+                weights(2);
+                arrive(0);
+                ptx::tmem_st_32x32b_x16(ts + 32, w);
+                weights(3);
+                arrive(1);
+                ptx::tmem_st_32x32b_x16(ts + 48, w);
+                arrive(2);
                 l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
             }
             if (!ok) break;
