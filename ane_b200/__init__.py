@@ -517,6 +517,8 @@ class Pages(ctypes.Structure):
 
 
 _DTYPES = {}  # torch dtype -> ANE_DTYPE_*
+_U64x6, _U64x12 = ctypes.c_uint64 * 6, ctypes.c_uint64 * 12  # two / four ane_rows one after another
+_byref = ctypes.byref
 
 
 def _dtype(t) -> int:
@@ -529,45 +531,66 @@ def _dtype(t) -> int:
         raise TypeError("expected float32, float16 or bfloat16, got %s" % t.dtype) from None
 
 
-def _rows(name: str, t, heads=None, dim=None) -> Rows:
-    """ane_rows of a CUDA tensor [tokens, heads, dim] whose last dimension is contiguous."""
+_raw_stream = None
+
+
+def _stream_of(stream, t) -> int:
+    """The cudaStream_t of `stream`, or of the current stream of t's device, which
+    has to be the current device."""
+    global _raw_stream
+    torch = _torch()
+    device = t.get_device()
+    if device != torch.cuda.current_device():
+        raise ValueError("the tensors are on device %d, the current device is %d" % (device, torch.cuda.current_device()))
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is None:  # a Stream object per call costs 3 us
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
+
+
+def _rows(name: str, t, heads=None, dim=None):
+    """(address, token stride, head stride) of a CUDA tensor [tokens, heads, dim]
+    whose last dimension is contiguous."""
     if t.dim() != 3 or not t.is_cuda:
         raise ValueError("%s must be a CUDA tensor [tokens, heads, dim]" % name)
-    _, h, d = t.shape
-    if (heads is not None and h != heads) or (dim is not None and d != dim):
-        raise ValueError("%s has heads x dim %d x %d, expected %s x %s" % (name, h, d, heads, dim))
+    if heads is not None and t.shape[1:] != (heads, dim):
+        raise ValueError("%s has heads x dim %s, expected %d x %d" % (name, tuple(t.shape[1:]), heads, dim))
     st, sh, sd = t.stride()
-    if sd != 1 and d > 1:
+    if sd != 1 and t.shape[2] > 1:
         raise ValueError("%s: the last dimension must be contiguous" % name)
-    return Rows(t.data_ptr(), st, sh)
+    if st < 0 or sh < 0:
+        raise ValueError("%s: negative strides" % name)
+    return t.data_ptr(), st, sh
 
 
 def _i32_vector(name: str, t, n=None) -> int:
-    torch = _torch()
-    if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
+    if t.dtype is not _torch().int32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
         raise ValueError("%s must be a contiguous int32 CUDA vector" % name)
     if n is not None and t.numel() != n:
         raise ValueError("%s has %d entries, expected %d" % (name, t.numel(), n))
     return t.data_ptr()
 
 
-def _output(name: str, out, like, out_dtype, stream):
+def _output(out, like, out_dtype, stream):
     """`out` or a new tensor of like's shape; a new one is kept alive for `stream`."""
-    torch = _torch()
     if out is None:
-        out = torch.empty(like.shape, dtype=out_dtype or like.dtype, device=like.device)
+        if out_dtype is None:
+            out = _torch().empty_like(like, memory_format=_torch().contiguous_format)
+        else:
+            out = _torch().empty(like.shape, dtype=out_dtype, device=like.device)
         if stream is not None:
             out.record_stream(stream)
     elif out.shape != like.shape:
-        raise ValueError("%s must have the shape of q" % name)
+        raise ValueError("out must have the shape of q")
     return out
 
 
 def _lse_ptr(lse, q):
     if lse is None:
         return None
-    torch = _torch()
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or not lse.is_cuda:
+    if lse.dtype is not _torch().float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or not lse.is_cuda:
         raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, heads]")
     return lse.data_ptr()
 
@@ -580,27 +603,29 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     of a sequence sees its last key.  scale defaults to dim ** -0.5; out_dtype
     may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp."""
     T, heads, dim = q.shape
-    kv_heads = k.shape[1]
-    if v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
+    Tk, kv_heads, _ = k.shape
+    if v.shape != k.shape or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError("k and v must have one shape and q's dtype")
     n_seq = cu_q.numel() - 1
     if n_seq < 0:
         raise ValueError("cu_q needs n_seq + 1 entries")
-    out = _output("out", out, q, out_dtype, stream)
-    rq, rk, rv, ro = _rows("q", q), _rows("k", k, kv_heads, dim), _rows("v", v), _rows("out", out)
-    check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, k.shape[0],
-                                   dim ** -0.5 if scale is None else float(scale), ctypes.byref(rq), ctypes.byref(rk),
-                                   ctypes.byref(rv), _i32_vector("cu_q", cu_q),
+    if cu_k is None and Tk != T:
+        raise ValueError("without cu_k, k and v must have as many rows as q")
+    rq, rk, rv = _rows("q", q), _rows("k", k, kv_heads, dim), _rows("v", v)
+    out = _output(out, q, out_dtype, stream)
+    rows = _U64x12(*rq, *rk, *rv, *_rows("out", out))
+    check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, Tk,
+                                   dim ** -0.5 if scale is None else scale, _byref(rows), _byref(rows, 24),
+                                   _byref(rows, 48), _i32_vector("cu_q", cu_q),
                                    None if cu_k is None else _i32_vector("cu_k", cu_k, n_seq + 1), _dtype(out),
-                                   ctypes.byref(ro), _lse_ptr(lse, q), _stream_ptr(stream)))
+                                   _byref(rows, 72), _lse_ptr(lse, q), _stream_of(stream, q)))
     return out
 
 
 def attn_decode_workspace(batch: int, heads: int, kv_heads: int, dim: int, device="cuda"):
-    """Workspace for attn_decode calls of up to these sizes on one stream."""
-    torch = _torch()
+    """Workspace for attn_decode calls of these sizes, one at a time."""
     n = int(_lib.ane_attn_decode_workspace_size(batch, heads, kv_heads, dim))
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return _torch().empty(n, dtype=_torch().uint8, device=device)
 
 
 def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, out=None, out_dtype=None, lse=None,
@@ -610,28 +635,28 @@ def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, 
     tables int32 [n_slots, max_pages], lens int32 [n_slots], row b of the batch
     in slot slots[b] (default b).  The first `shared` tokens are the same for the
     whole batch and are read once, through the pages of row 0's slot."""
-    torch = _torch()
     B, heads, dim = q.shape
-    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError("k and v must be [pages, page_tokens, kv_heads, dim] of one layout and q's dtype")
     pages, page_tokens, kv_heads, kd = k.shape
-    sp, st, sh, sd = k.stride()
+    sp, st, sh, sd = strides = k.stride()
+    if v.shape != k.shape or v.stride() != strides or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise ValueError("k and v must be [pages, page_tokens, kv_heads, dim] of one layout and q's dtype")
     if kd != dim or (sd != 1 and dim > 1) or not k.is_cuda or not v.is_cuda:
         raise ValueError("k and v must be CUDA tensors of q's dim, contiguous in it")
-    if tables.dim() != 2 or tables.dtype != torch.int32 or not tables.is_cuda or not tables.is_contiguous():
+    if tables.dim() != 2 or tables.dtype is not _torch().int32 or not tables.is_cuda or not tables.is_contiguous():
         raise ValueError("tables must be a contiguous int32 CUDA tensor [n_slots, max_pages]")
     n_slots, max_pages = tables.shape
+    rq = _rows("q", q)
     if workspace is None:
         workspace = attn_decode_workspace(B, heads, kv_heads, dim, q.device)
         if stream is not None:
             workspace.record_stream(stream)
-    out = _output("out", out, q, out_dtype, stream)
-    rq, ro = _rows("q", q), _rows("out", out)
+    out = _output(out, q, out_dtype, stream)
+    rows = _U64x6(*rq, *_rows("out", out))
     pg = Pages(k.data_ptr(), v.data_ptr(), pages, page_tokens, sp, st, sh)
-    check(_lib.ane_attn_decode_dev(_dtype(q), B, heads, kv_heads, dim, dim ** -0.5 if scale is None else float(scale),
-                                   ctypes.byref(rq), ctypes.byref(pg), tables.data_ptr(), n_slots, max_pages,
+    check(_lib.ane_attn_decode_dev(_dtype(q), B, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale,
+                                   _byref(rows), _byref(pg), tables.data_ptr(), n_slots, max_pages,
                                    _i32_vector("lens", lens, n_slots),
                                    None if slots is None else _i32_vector("slots", slots, B), shared, _dtype(out),
-                                   ctypes.byref(ro), _lse_ptr(lse, q), workspace.data_ptr(), workspace.numel(),
-                                   _stream_ptr(stream)))
+                                   _byref(rows, 24), _lse_ptr(lse, q), workspace.data_ptr(), workspace.numel(),
+                                   _stream_of(stream, q)))
     return out

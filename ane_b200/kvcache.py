@@ -77,7 +77,7 @@ class KVCache:
         granted = self._granted(granted, n, stream)
         ane.check(ane.lib.ane_kv_reserve_dev(self._ref, n, ane._i32_vector("slots", slots),
                                              ane._i32_vector("counts", counts, n),
-                                             ane._i32_vector("granted", granted, n), ane._stream_ptr(stream)))
+                                             ane._i32_vector("granted", granted, n), ane._stream_of(stream, self.k)))
         return granted
 
     def write(self, layer: int, slots, k, v, cu=None, granted=None, stream=None) -> None:
@@ -85,14 +85,14 @@ class KVCache:
         cache's type; cu None: one row per slot) become the last tokens of
         slots[i] on `layer`; rows of requests that were not granted are dropped."""
         n = slots.numel()
-        rk, rv = ane._rows("k", k, self.kv_heads, self.dim), ane._rows("v", v, self.kv_heads, self.dim)
+        rows = ane._U64x6(*ane._rows("k", k, self.kv_heads, self.dim), *ane._rows("v", v, self.kv_heads, self.dim))
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape and dtype")
         ane.check(ane.lib.ane_kv_write_dev(self._ref, layer, n, ane._i32_vector("slots", slots),
                                            None if cu is None else ane._i32_vector("cu", cu, n + 1),
                                            None if granted is None else ane._i32_vector("granted", granted, n),
-                                           k.shape[0], ane._dtype(k), ctypes.byref(rk), ctypes.byref(rv),
-                                           ane._stream_ptr(stream)))
+                                           k.shape[0], ane._dtype(k), ctypes.byref(rows), ctypes.byref(rows, 24),
+                                           ane._stream_of(stream, self.k)))
 
     def fork(self, parents, children, granted=None, stream=None):
         """children[i] (empty slots) become copies of parents[i]; returns granted."""
@@ -100,13 +100,13 @@ class KVCache:
         granted = self._granted(granted, n, stream)
         ane.check(ane.lib.ane_kv_fork_dev(self._ref, n, ane._i32_vector("parents", parents, n),
                                           ane._i32_vector("children", children),
-                                          ane._i32_vector("granted", granted, n), ane._stream_ptr(stream)))
+                                          ane._i32_vector("granted", granted, n), ane._stream_of(stream, self.k)))
         return granted
 
     def free(self, slots, stream=None) -> None:
         """The slots give up their pages and are empty."""
         ane.check(ane.lib.ane_kv_free_dev(self._ref, slots.numel(), ane._i32_vector("slots", slots),
-                                          ane._stream_ptr(stream)))
+                                          ane._stream_of(stream, self.k)))
 
     def copy_pages(self, src, dst, into: "KVCache | None" = None, stream=None) -> None:
         """Pages src[i] to pages dst[i] on all layers (of `into`, or of this
@@ -114,7 +114,7 @@ class KVCache:
         to = self if into is None else into
         n = src.numel()
         ane.check(ane.lib.ane_kv_copy_pages_dev(self._ref, to._ref, n, ane._i32_vector("src", src),
-                                                ane._i32_vector("dst", dst, n), ane._stream_ptr(stream)))
+                                                ane._i32_vector("dst", dst, n), ane._stream_of(stream, self.k)))
 
     def compact(self, refs_out=None, tables_out=None, remap=None, live=None, stream=None):
         """Moves the pages in use to the lowest numbers.  Returns (live, remap):
@@ -134,7 +134,7 @@ class KVCache:
             raise ValueError("tables_out must be a contiguous int32 tensor of the tables' shape")
         ane.check(ane.lib.ane_kv_compact_dev(self._ref, ane._i32_vector("refs_out", refs_out, self.pages),
                                              tables_out.data_ptr(), ane._i32_vector("remap", remap, self.pages),
-                                             ane._i32_vector("live", live, 1), ane._stream_ptr(stream)))
+                                             ane._i32_vector("live", live, 1), ane._stream_of(stream, self.k)))
         return live, remap
 
     def attend(self, layer: int, q, slots=None, shared: int = 0, **kw):
