@@ -127,8 +127,9 @@ SIGNATURES = {
     "ane_ipc_get_handle": (_i32, [_vp, _vp, _vp]),
     "ane_ipc_open_handle": (_i32, [_vp, _vp]),
     "ane_ipc_close_handle": (_i32, [_vp]),
+    "ane_attn_prompt_workspace_size": (_sz, [_u32, _u32, _u32, _u32, _u32, _u32]),
     "ane_attn_prompt_dev": (_i32, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _f, _vp, _vp, _vp, _vp, _vp, _u32, _vp,
-                                   _vp, _vp]),
+                                   _vp, _vp, _sz, _vp]),
     "ane_attn_decode_workspace_size": (_sz, [_u32, _u32, _u32, _u32]),
     "ane_attn_decode_dev": (_i32, [_u32, _u32, _u32, _u32, _u32, _f, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _u32, _u32,
                                    _vp, _vp, _vp, _sz, _vp]),
@@ -595,13 +596,15 @@ def _lse_ptr(lse, q):
     return lse.data_ptr()
 
 
-def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, lse=None, stream=None):
+def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, lse=None, workspace=None, stream=None):
     """Causal attention over packed prompts: q [tokens, heads, dim], k and v
     [tokens, kv_heads, dim] (float16 or bfloat16, any token and head strides of
     whole 16 bytes), sequence s at rows cu_q[s]:cu_q[s+1] of q and
     cu_k[s]:cu_k[s+1] of k and v (int32; cu_k defaults to cu_q).  The last query
     of a sequence sees its last key.  scale defaults to dim ** -0.5; out_dtype
-    may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp."""
+    may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp.
+    workspace: a uint8 tensor of ane_attn_prompt_workspace_size bytes (default: a
+    new one where the call needs any)."""
     T, heads, dim = q.shape
     Tk, kv_heads, _ = k.shape
     if v.shape != k.shape or k.dtype is not q.dtype or v.dtype is not q.dtype:
@@ -614,11 +617,20 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     rq, rk, rv = _rows("q", q), _rows("k", k, kv_heads, dim), _rows("v", v)
     out = _output(out, q, out_dtype, stream)
     rows = _U64x12(*rq, *rk, *rv, *_rows("out", out))
+    ws_ptr, ws_bytes = None, 0
+    if workspace is None:
+        ws_bytes = _lib.ane_attn_prompt_workspace_size(n_seq, heads, kv_heads, dim, T, Tk)
+        if ws_bytes:
+            workspace = _torch().empty(ws_bytes, dtype=_torch().uint8, device=q.device)
+            if stream is not None:
+                workspace.record_stream(stream)
+    if workspace is not None:
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
     check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, Tk,
                                    dim ** -0.5 if scale is None else scale, _byref(rows), _byref(rows, 24),
                                    _byref(rows, 48), _i32_vector("cu_q", cu_q),
                                    None if cu_k is None else _i32_vector("cu_k", cu_k, n_seq + 1), _dtype(out),
-                                   _byref(rows, 72), _lse_ptr(lse, q), _stream_of(stream, q)))
+                                   _byref(rows, 72), _lse_ptr(lse, q), ws_ptr, ws_bytes, _stream_of(stream, q)))
     return out
 
 

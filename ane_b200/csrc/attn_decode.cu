@@ -542,7 +542,7 @@ struct PrefixJob {
         factor = l == 0.0f ? 0.0f : 1.0f;
     }
     __device__ uint32_t dim() const { return p.dim; }
-    __device__ uint32_t out_dtype() const { return ANE_DTYPE_F32; }
+    __device__ uint32_t out_dtype(const BigItem&) const { return ANE_DTYPE_F32; }
 };
 
 template <typename T, int DP>

@@ -88,59 +88,74 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Stores that stay predicated: a branch around each cost more than the store.
+__device__ __forceinline__ void store16_if(bool on, void* dst, uint4 v) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %0, 0;\n\t"
+        "@p st.global.v4.b32 [%1], {%2, %3, %4, %5};\n\t}" ::"r"((int)on),
+        "l"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+        : "memory");
+}
 // One warp: the DP accumulator columns of its 32 rows (TMEM address `to`), times
-// factor, to each row's dst (NULL: no such row), rounded to out_dtype.  128 bytes
+// factor, to each row's dst (NULL: no such row), as T or F32.  128 bytes
 // of every row at a time go through shared memory, so that a store instruction
 // writes four rows' whole lines (a row per lane would touch 32 lines).
 // any: false if there is no accumulator (the rows are 0).
-template <int DP>
+template <typename T>
+__device__ __forceinline__ uint32_t pack_out(uint32_t a, uint32_t b) {
+    return Type<T>::pack(__uint_as_float(a), __uint_as_float(b));
+}
+template <typename T, int DP>
 __device__ __forceinline__ void store_rows(uint8_t* stage, uint8_t* dst, float factor, bool any, uint32_t to,
                                            uint32_t dim, uint32_t out_dtype) {
     const int lane = threadIdx.x & 31;
-    const int cols = out_dtype == ANE_DTYPE_F32 ? 32 : 64;
-    const uint32_t row_bytes = dim * (out_dtype == ANE_DTYPE_F32 ? 4 : 2);
-#pragma unroll 1
-    for (int c = 0; c < DP; c += cols) {
-#pragma unroll 1
-        for (int half = 0; half < cols / 32; half++) {
-            uint32_t o[32];
-            if (any) {
-                ptx::tmem_ld_32x32b_x32(to + c + half * 32, o);
-                ptx::tmem_ld_wait();
-                ptx::pin32(o);
-            }
-            const bool zero = !any || factor == 0.0f;  // whatever the accumulator holds
-#pragma unroll
-            for (int i = 0; i < 32; i++) o[i] = zero ? 0u : __float_as_uint(__uint_as_float(o[i]) * factor);
-            auto put = [&](int chunk, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
-                *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = make_uint4(a, b, d, e);
-            };
-            if (out_dtype == ANE_DTYPE_F32) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) put(i, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float x = __uint_as_float(o[8 * i + 2 * k]), y = __uint_as_float(o[8 * i + 2 * k + 1]);
-                        w[k] = out_dtype == ANE_DTYPE_F16 ? Type<__half>::pack(x, y) : Type<__nv_bfloat16>::pack(x, y);
-                    }
-                    put(half * 4 + i, w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
+    const uint32_t row_bytes = dim * (out_dtype == ANE_DTYPE_F32 ? 4 : 2), at0 = (lane & 7) * 16;
+    const bool zero = !any || factor == 0.0f;  // whatever the accumulator holds
+    const unsigned long long d = reinterpret_cast<unsigned long long>(dst);
+    uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
+    auto flush = [&](uint32_t at) {  // the staged 128 bytes go to byte `at` of the rows
         __syncwarp();
-        const uint32_t at = (uint32_t)(c / cols) * 128 + (lane & 7) * 16;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int r = i * 4 + (lane >> 3);
-            uint8_t* d = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+            const unsigned long long dr = __shfl_sync(0xffffffffu, d, r);
             const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if (d && at < row_bytes) *reinterpret_cast<uint4*>(d + at) = v;
+            store16_if(dr && at + at0 < row_bytes, reinterpret_cast<uint8_t*>(dr) + at + at0, v);
         }
         __syncwarp();
+    };
+#pragma unroll 1
+    for (int c = 0; c < DP; c += 64) {
+        // one wait for 64 columns: each costs some 350 cycles next to running MMAs
+        // (read even if there is nothing: a branch here made the compiler spill)
+        uint32_t o[2][32];
+        ptx::tmem_ld_32x32b_x32(to + c, o[0]);
+        ptx::tmem_ld_32x32b_x32(to + c + 32, o[1]);
+        ptx::tmem_ld_wait();
+        ptx::pin32(o[0]);
+        ptx::pin32(o[1]);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[h][i] = zero ? 0u : __float_as_uint(__uint_as_float(o[h][i]) * factor);
+        if (out_dtype == ANE_DTYPE_F32) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    mine[i ^ (lane & 7)] = make_uint4(o[h][4 * i], o[h][4 * i + 1], o[h][4 * i + 2], o[h][4 * i + 3]);
+                flush((c + h * 32) * 4);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t* x = &o[i >> 2][8 * (i & 3)];
+                mine[i ^ (lane & 7)] = make_uint4(pack_out<T>(x[0], x[1]), pack_out<T>(x[2], x[3]),
+                                                  pack_out<T>(x[4], x[5]), pack_out<T>(x[6], x[7]));
+            }
+            flush(c * 2);
+        }
     }
 }
 
@@ -151,7 +166,7 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, uint8_t* dst, float f
 //   visible(item, token)        keys that query token `token` of the item sees
 //   result(item, row, token, m, l, shift, dst, factor)  where a row's result goes, what it is
 //                               multiplied by (0: it is 0), its statistics written
-//   out_dtype(), dim()
+//   out_dtype(item), dim()
 template <typename T, int DP, class Job>
 __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CUtensorMap* map_k,
                                               const CUtensorMap* map_v, uint32_t group, float scale2, int* err,
@@ -381,12 +396,15 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
         const bool real = row < tile_tokens * (int)group;
         uint32_t sc = 0, oc = 0;
         bool ok = true;
-        BigItem it;
-        for (int i = 0; ok && take(i, it); i++) {
-            const bool mine = real && token < it.tokens;
-            const int vis = mine ? job.visible(it, token) : 0;
+        for (int i = 0; ok; i++) {
+            const int e = i % kItemRing;
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.item_full[e], (i / kItemRing) & 1, err));
+            const BigItem& it = sm.items[e];  // stays there until this warp is done with it
+            if (!ok || it.head < 0) break;
+            const int begin = it.begin, end = it.end[t];
+            const int vis = real && token < it.tokens ? job.visible(it, token) : 0;
             float m = kNegInf, l = 0.0f;
-            for (int j = it.begin; j < it.end[t]; j++) {
+            for (int j = begin; j < end; j++) {
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.s_full[t], sc & 1, err));
                 if (!ok) break;
                 sc++;
@@ -424,7 +442,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 auto raise = [&](float top) {
                     const float mn = fmaxf(m, top), base = mn == kNegInf ? 0.0f : mn;
                     const float c = exp2_fast(m - base);
-                    if (j > it.begin) {
+                    if (j > begin) {
 #pragma unroll 1
                         for (int x = 0; x < DP; x += 32) {
                             uint32_t o[32];
@@ -447,7 +465,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 };
                 const int rest = vis - j * kBigKeys;  // keys of this tile that the row sees
                 float top;
-                if (j > it.begin && __all_sync(0xffffffffu, rest >= kBigKeys)) {
+                if (j > begin && __all_sync(0xffffffffu, rest >= kBigKeys)) {
                     // The reference of the tiles before will do for this one too,
                     // nearly always: its first weights are under way before the
                     // tile's maximum is known.
@@ -494,7 +512,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
             }
             if (!ok) break;
-            if (it.begin < it.end[t]) {
+            if (begin < end) {
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.o_full[t], oc & 1, err));
                 if (!ok) break;
                 oc++;
@@ -502,9 +520,11 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
             }
             uint8_t* dst = nullptr;
             float factor = 0.0f;
-            if (mine) job.result(it, row, token, m, l, kShift, dst, factor);
-            store_rows<DP>(sm.out[warp], dst, factor, it.begin < it.end[t], to, job.dim(), job.out_dtype());
+            if (real && token < it.tokens) job.result(it, row, token, m, l, kShift, dst, factor);
+            store_rows<T, DP>(sm.out[warp], dst, factor, begin < end, to, job.dim(), job.out_dtype(it));
             ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&sm.item_empty[e]);
         }
     }
     ptx::tc_fence_before();

@@ -459,11 +459,15 @@ typedef struct ane_rows {
  * sequence are never part of a result, whatever they hold.  lse (NULL to skip)
  * receives [total_q][heads] natural logarithms of the softmax sums.
  * dim % 8 == 0, dim <= 128; heads a multiple of kv_heads, at most 64 per
- * kv_head; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold. */
+ * kv_head; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold.
+ * workspace: 256-byte aligned, ane_attn_prompt_workspace_size bytes (which may be
+ * 0), any contents, not shared by calls that may overlap. */
+size_t ane_attn_prompt_workspace_size(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                                      uint32_t total_q, uint32_t total_k);
 int ane_attn_prompt_dev(uint32_t dtype, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                         uint32_t total_q, uint32_t total_k, float scale, const ane_rows* q, const ane_rows* k,
                         const ane_rows* v, const int32_t* cu_q, const int32_t* cu_k, uint32_t out_dtype,
-                        const ane_rows* out, float* lse, void* stream);
+                        const ane_rows* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* A layer's pages: element e of head h of token t of page p is
  * k[p * page_stride + t * token_stride + h * head_stride + e] (v alike;

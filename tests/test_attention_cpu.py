@@ -20,7 +20,7 @@ def rows(data=A, token=512, head=64):
 def prompt(dtype=1, n=1, heads=4, kv_heads=2, dim=64, tq=10, tk=10, q=None, k=None, v=None, cu=A, out_dtype=1, out=None):
     q, k, v, out = (rows() if r is None else r for r in (q, k, v, out))
     return L.ane_attn_prompt_dev(dtype, n, heads, kv_heads, dim, tq, tk, 0.1, P(q), P(k), P(v), cu, None, out_dtype,
-                                 P(out), None, None)
+                                 P(out), None, None, 0, None)
 
 
 def decode(dtype=1, batch=2, heads=4, kv_heads=2, dim=64, q=None, pages=None, n_slots=4, max_pages=8, shared=0,
@@ -105,6 +105,14 @@ def test_no_gpu_means_loud_failure():
         pytest.skip("a GPU is present")
     assert prompt() == NO_DEVICE and prompt(n=0) == NO_DEVICE and decode() == NO_DEVICE
     assert all(rc == NO_DEVICE for rc in calls(cache()))
+
+
+def test_prompt_workspace():
+    f = L.ane_attn_prompt_workspace_size
+    assert f(1, 32, 32, 128, 17, 17) == 0  # nothing to split
+    n = f(1, 32, 8, 128, 512, 8192)
+    assert n > 0 and n % 256 == 0
+    assert prompt(n=1, heads=32, kv_heads=8, dim=128, tq=512, tk=8192) == INVALID  # no workspace given
 
 
 def test_workspace_size():

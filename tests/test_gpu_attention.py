@@ -95,6 +95,32 @@ def test_prompt_history_and_empty_rows(ane, lq, lk, dtype):
     prompt_case(ane, lq, lk, 2, 2, 64, dtype, out_dtype=F32)
 
 
+@pytest.mark.parametrize("lq,lk,heads,kv_heads,dim,dtype", [
+    ([1], [5000], 8, 8, 128, F16),               # one token against a long history: every item cut many times
+    ([3, 0, 1], [40000, 0, 70], 4, 1, 64, BF16),
+    ([100, 513, 64], [2100, 513, 1000], 8, 2, 128, BF16),
+    ([2000], [1100], 4, 4, 128, F16),            # the first 900 queries see nothing
+    ([1500, 900, 0, 700], [1500, 900, 0, 700], 6, 2, 80, F16),
+    ([300] * 7, [1000 + 100 * i for i in range(7)], 16, 2, 64, F16),
+    ([260], [8200], 5, 1, 128, BF16),
+])
+def test_prompt_few_items_cut_along_the_keys(ane, lq, lk, heads, kv_heads, dim, dtype):
+    prompt_case(ane, lq, lk, heads, kv_heads, dim, dtype)
+    prompt_case(ane, lq, lk, heads, kv_heads, dim, dtype, out_dtype=F32, want_lse=False, seed=1)
+
+
+def test_prompt_cut_items_repeat(ane):
+    """The joined parts do not depend on scheduling, nor on what the workspace holds."""
+    q, k, v, cq, ck, out = prompt_case(ane, [200, 90], [6000, 3000], 8, 2, 128, F16)
+    ws = torch.empty(ane.lib.ane_attn_prompt_workspace_size(2, 8, 2, 128, q.shape[0], k.shape[0]), dtype=torch.uint8,
+                     device="cuda")
+    assert ws.numel() > 0
+    for _ in range(3):
+        ws.random_(0, 255)
+        got = ane.attn_prompt(q, k, v, i32(cq), i32(ck), workspace=ws)
+        assert torch.equal(got[cq[0]:cq[-1]], out[cq[0]:cq[-1]])
+
+
 def test_prompt_large_scores(ane):
     """Scores of several hundred: the maximum moves far from tile to tile."""
     prompt_case(ane, [600], [600], 2, 1, 128, F16, spread=60.0)
@@ -130,7 +156,7 @@ def test_prompt_neighbours_may_hold_anything(ane):
 
 
 def test_prompt_batch_invariant_and_repeatable(ane):
-    """A sequence's bits do not depend on what it is packed with, nor on the run."""
+    """Whole items: a sequence's bits do not depend on what it is packed with, nor on the run."""
     lens = [300, 17, 411]
     q, k, v, cq, _, out = prompt_case(ane, lens, lens, 8, 2, 128, BF16, seed=5)
     again = ane.attn_prompt(q, k, v, i32(cq))
