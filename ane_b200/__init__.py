@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import functools
 import os
 import struct
 
@@ -596,6 +597,11 @@ def _lse_ptr(lse, q):
     return lse.data_ptr()
 
 
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace_size(*sizes) -> int:
+    return int(_lib.ane_attn_prompt_workspace_size(*sizes))
+
+
 def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, lse=None, workspace=None, stream=None):
     """Causal attention over packed prompts: q [tokens, heads, dim], k and v
     [tokens, kv_heads, dim] (float16 or bfloat16, any token and head strides of
@@ -619,7 +625,7 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     rows = _U64x12(*rq, *rk, *rv, *_rows("out", out))
     ws_ptr, ws_bytes = None, 0
     if workspace is None:
-        ws_bytes = _lib.ane_attn_prompt_workspace_size(n_seq, heads, kv_heads, dim, T, Tk)
+        ws_bytes = _prompt_workspace_size(n_seq, heads, kv_heads, dim, T, Tk)
         if ws_bytes:
             workspace = _torch().empty(ws_bytes, dtype=_torch().uint8, device=q.device)
             if stream is not None:

@@ -29,8 +29,9 @@ constexpr uint32_t kBigBlocks = 148;   // of prefix_kernel, about
 constexpr int kTile = 64;              // tokens per key/value tile
 constexpr int kThreads = 160;          // four computing warps and the producer
 constexpr int kJoinThreads = 128;
+constexpr uint32_t kKept = 256;        // sequences whose slot and length stay in shared memory
 constexpr int kUnits = 2;              // units announced ahead
-constexpr int kUnitCost = 1;           // a unit's start and end cost about what a tile does
+constexpr int kUnitCost = 2;           // a unit's start and end cost about what two tiles do
 
 struct Params {
     uint32_t batch, heads, kv_heads, group, dim, out_dtype;
@@ -54,10 +55,12 @@ __device__ __forceinline__ int slot_of(const Params& p, uint32_t b) {
     const int s = p.slots ? __ldcg(p.slots + b) : (int)b;
     return s >= 0 && (uint32_t)s < p.n_slots ? s : -1;
 }
-__device__ __forceinline__ int len_of(const Params& p, uint32_t b) {
+// {slot, tokens} of sequence b; no slot: {-1, 0}
+__device__ __forceinline__ int2 seq_of(const Params& p, uint32_t b) {
     const int s = slot_of(p, b);
-    return s < 0 ? 0 : min(max(__ldcg(p.lens + s), 0), (int)(p.max_pages << p.page_shift));
+    return make_int2(s, s < 0 ? 0 : min(max(__ldcg(p.lens + s), 0), (int)(p.max_pages << p.page_shift)));
 }
+__device__ __forceinline__ int len_of(const Params& p, uint32_t b) { return seq_of(p, b).y; }
 // Own tiles start where the box of tokens does that holds the first own one.
 __device__ __forceinline__ int own_base(const Params& p) { return (int)(p.shared & ~(p.box_keys - 1)); }
 __device__ __forceinline__ int own_tiles(const Params& p, int len) {
@@ -90,6 +93,7 @@ struct DecodeSmem {
     int vis[kUnits][16];             // keys that count for each row, from the unit's lo
     float2 ml[kStages][4][16];       // {m, l} of each warp's rows
     int cum[kMaxBatch + 1];          // steps of the own units of the sequences before b, per head
+    int2 seq[kKept];                 // {slot, len} of the first sequences
     Unit unit[kUnits];
     uint64_t full[kStages], empty[kStages], joined[kStages], unit_full[kUnits], unit_empty[kUnits];
 };
@@ -230,7 +234,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         ptx::griddep_launch_dependents();
         ptx::griddep_wait();
     }
-    for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) sm.cum[b] = steps(own_tiles(p, len_of(p, b)));
+    for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) {
+        const int2 q = seq_of(p, b);
+        if (b < kKept) sm.seq[b] = q;
+        sm.cum[b] = steps(own_tiles(p, q.y));
+    }
+    auto seq = [&](uint32_t b) { return b < kKept ? sm.seq[b] : seq_of(p, b); };
     __syncthreads();
     if (warp == 0) {
         int base = 0;
@@ -284,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                         const int mid = (lo + hi + 1) >> 1;
                         if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1;
                     }
-                    if (lo != b_now) len_now = len_of(p, lo), b_now = lo;
+                    if (lo != b_now) len_now = seq((uint32_t)lo).y, b_now = lo;
                     u.prefix = 0;
                     u.b = lo;
                     n = sm.cum[lo + 1] - sm.cum[lo];
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             if (lane < 16) {
                 const uint32_t flat = (uint32_t)u.rt * 16 + lane;
-                sm.vis[e][lane] = flat >= rows ? 0 : u.prefix ? min(len_of(p, flat / p.group), (int)p.shared) : u.kend - u.lo;
+                sm.vis[e][lane] = flat >= rows ? 0 : u.prefix ? min(seq(flat / p.group).y, (int)p.shared) : u.kend - u.lo;
             }
         };
         auto announce = [&](const Unit& u) {
@@ -345,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int box = is_v ? lane - boxes : lane;
         const int key0 = box / kHalves * (int)p.box_keys, half = box % kHalves;
         auto table_of = [&](const Unit& x) {
-            return p.tables + (size_t)max(slot_of(p, x.prefix ? 0 : (uint32_t)x.b), 0) * p.max_pages;
+            return p.tables + (size_t)max(seq(x.prefix ? 0 : (uint32_t)x.b).x, 0) * p.max_pages;
         };
         auto entry = [&](const int32_t* table, int j, int kend) {  // page number of this lane's box
             return lane_on && j < kend ? __ldcg(table + min((uint32_t)j >> p.page_shift, p.max_pages - 1)) : 0;
