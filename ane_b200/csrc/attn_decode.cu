@@ -753,7 +753,13 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.batch = batch, p.heads = heads, p.kv_heads = kv_heads, p.group = heads / kv_heads, p.dim = dim;
     p.out_dtype = out_dtype;
     p.shared = shared;
-    const bool big = shared > 0 && (size_t)batch * p.group > 16;
+    // decode_kernel goes over the prefix once per 16 rows.  The second time costs
+    // little (L2), every further one a tile's time: prefix_kernel from where that
+    // makes eight tiles a block.  128 rows x 8 heads, 4096 shared: 31 us without it,
+    // 25 with it; 1024 shared: 23 and 23; 64 rows x 32 heads, 1024 shared: 41 and 44;
+    // 32 rows x 32 heads, 16384 shared: 74 and 86.
+    const uint64_t again = l.prefix_rts > 2 ? (uint64_t)(l.prefix_rts - 2) * kv_heads * ceil_div(shared, kTile) : 0;
+    const bool big = again >= 8 * 2 * (uint64_t)kBigBlocks;
     if (big) {
         const uint32_t tiles = (uint32_t)ceil_div(shared, kBigKeys);
         p.big_splits = l.big_splits < tiles ? l.big_splits : tiles;

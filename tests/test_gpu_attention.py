@@ -335,3 +335,15 @@ def test_decode_long_cache_offsets(ane):
 
 def test_decode_full_batch(ane):
     decode_case(ane, [100 + b % 40 for b in range(1024)], 96, 2, 1, 64, 16, F16, want_lse=False)
+
+
+@pytest.mark.parametrize("lens,shared,heads,kv_heads,dim,page,dtype", [
+    ([2600 + 13 * b for b in range(33)], 2600, 16, 2, 128, 64, BF16),     # 264 rows: a full pair and a few rows
+    ([4100 + b for b in range(70)] + [0, 100, 4096], 4096, 8, 8, 64, 16, F16),
+    ([1500 + 50 * (b % 9) for b in range(130)], 1411, 20, 4, 80, 8, F16),  # 5 heads a group: 125 rows per tile
+    ([2048] * 64, 2048, 32, 8, 128, 256, BF16),                           # nothing of their own
+])
+def test_decode_long_prefix_many_rows(ane, lens, shared, heads, kv_heads, dim, page, dtype):
+    decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype)
+    decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype, out_dtype=F32, want_lse=False, seed=2,
+                layout="heads")
