@@ -518,38 +518,47 @@ class Pages(ctypes.Structure):
                 ("head_stride", ctypes.c_size_t)]
 
 
-_DTYPES = {}  # torch dtype -> ANE_DTYPE_*
 _U64x6, _U64x12 = ctypes.c_uint64 * 6, ctypes.c_uint64 * 12  # two / four ane_rows one after another
 _byref = ctypes.byref
 
 
-def _dtype(t) -> int:
-    if not _DTYPES:
+class _Bound:
+    """What the bindings below use of torch, looked up once (a small attention
+    takes a few microseconds on the device: the host must not take many more)."""
+    torch = None
+
+    @classmethod
+    def bind(cls):
         torch = _torch()
-        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise TypeError("expected float32, float16 or bfloat16, got %s" % t.dtype) from None
+        cls.i32, cls.f32 = torch.int32, torch.float32
+        cls.dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # ANE_DTYPE_*
+        cls.empty, cls.empty_like, cls.current_device = torch.empty, torch.empty_like, torch.cuda.current_device
+        # the handle without a Stream object, which costs 3 us
+        cls.raw_stream = staticmethod(getattr(torch._C, "_cuda_getCurrentRawStream", None) or
+                                      (lambda d: torch.cuda.current_stream(d).cuda_stream))
+        cls.torch = torch
 
 
-_raw_stream = None
+def _bound():
+    if _Bound.torch is None:
+        _Bound.bind()
+    return _Bound
+
+
+def _dtype(t) -> int:
+    code = _bound().dtypes.get(t.dtype)
+    if code is None:
+        raise TypeError("expected float32, float16 or bfloat16, got %s" % t.dtype)
+    return code
 
 
 def _stream_of(stream, t) -> int:
     """The cudaStream_t of `stream`, or of the current stream of t's device, which
     has to be the current device."""
-    global _raw_stream
-    torch = _torch()
-    device = t.get_device()
-    if device != torch.cuda.current_device():
-        raise ValueError("the tensors are on device %d, the current device is %d" % (device, torch.cuda.current_device()))
-    if stream is not None:
-        return stream.cuda_stream
-    if _raw_stream is None:  # a Stream object per call costs 3 us
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-            lambda d: torch.cuda.current_stream(d).cuda_stream)
-    return _raw_stream(device)
+    device, current = t.get_device(), _bound().current_device()
+    if device != current:
+        raise ValueError("the tensors are on device %d, the current device is %d" % (device, current))
+    return _Bound.raw_stream(device) if stream is None else stream.cuda_stream
 
 
 def _rows(name: str, t, heads=None, dim=None):
@@ -557,18 +566,16 @@ def _rows(name: str, t, heads=None, dim=None):
     whose last dimension is contiguous."""
     if t.dim() != 3 or not t.is_cuda:
         raise ValueError("%s must be a CUDA tensor [tokens, heads, dim]" % name)
+    st, sh, sd = t.stride()
     if heads is not None and t.shape[1:] != (heads, dim):
         raise ValueError("%s has heads x dim %s, expected %d x %d" % (name, tuple(t.shape[1:]), heads, dim))
-    st, sh, sd = t.stride()
     if sd != 1 and t.shape[2] > 1:
         raise ValueError("%s: the last dimension must be contiguous" % name)
-    if st < 0 or sh < 0:
-        raise ValueError("%s: negative strides" % name)
     return t.data_ptr(), st, sh
 
 
 def _i32_vector(name: str, t, n=None) -> int:
-    if t.dtype is not _torch().int32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
+    if t.dtype is not _bound().i32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
         raise ValueError("%s must be a contiguous int32 CUDA vector" % name)
     if n is not None and t.numel() != n:
         raise ValueError("%s has %d entries, expected %d" % (name, t.numel(), n))
@@ -578,10 +585,8 @@ def _i32_vector(name: str, t, n=None) -> int:
 def _output(out, like, out_dtype, stream):
     """`out` or a new tensor of like's shape; a new one is kept alive for `stream`."""
     if out is None:
-        if out_dtype is None:
-            out = _torch().empty_like(like, memory_format=_torch().contiguous_format)
-        else:
-            out = _torch().empty(like.shape, dtype=out_dtype, device=like.device)
+        # (empty_like alone would follow the strides of a view into fused rows)
+        out = _bound().empty(like.shape, dtype=out_dtype or like.dtype, device=like.device)
         if stream is not None:
             out.record_stream(stream)
     elif out.shape != like.shape:
@@ -592,7 +597,7 @@ def _output(out, like, out_dtype, stream):
 def _lse_ptr(lse, q):
     if lse is None:
         return None
-    if lse.dtype is not _torch().float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or not lse.is_cuda:
+    if lse.dtype is not _bound().f32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or not lse.is_cuda:
         raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, heads]")
     return lse.data_ptr()
 
