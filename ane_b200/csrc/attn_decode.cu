@@ -1,22 +1,23 @@
 // attn_decode.cu -- attention of one new token per sequence over a paged cache
 // whose sequences share a prefix.
 //
-// Two kinds of work.  The prefix meets all of the batch's query rows (batch x
-// heads of the group, per key/value head); each sequence's own tokens meet only
-// its group of rows.
+// decode_kernel works on units of at most 16 query rows (as many sequences as
+// fit, with the heads that share a key/value head) on mma.sync: a unit's keys are
+// the shared prefix, which all of its rows see, and then each of its sequences'
+// own tokens, which only that sequence's rows see.  It is bound by the bytes of K
+// and V, so all units' 64-token tiles are laid end to end and cut into equal
+// spans, one per block: ragged lengths and a single long sequence load the chip
+// alike.  Two producer warps stream a span's tiles through a ring by TMA, across
+// unit boundaries (a warp issues its lanes' boxes one by one, about 50 ns each:
+// with pages of 16 a tile is 16 boxes), while four warps compute, each a quarter
+// of a tile's tokens.
 //
-// decode_kernel does units of at most 16 rows on mma.sync: the own tokens, and
-// the prefix while the batch has few rows.  It is bound by the bytes of K and V,
-// so all units' 64-token tiles are laid end to end and cut into equal spans, one
-// per block: ragged lengths and a single long sequence load the chip alike.  A
-// producer warp streams a span's tiles through a ring by TMA, across unit
-// boundaries, while four warps compute (each a quarter of a tile's tokens).
-//
-// prefix_kernel does the prefix of a batch with more rows on tcgen05
-// (attn_sm100.cuh), 256 rows against every key tile.
+// Every unit reads the prefix again.  With many rows prefix_kernel does the prefix
+// instead, on tcgen05 (attn_sm100.cuh), 256 rows against every key tile.
 //
 // Both leave unnormalised partial results (m, l, o); join_kernel adds them per
-// output row in a fixed order, so results do not depend on scheduling.
+// output row in a fixed order, so results do not depend on scheduling.  Where
+// units are known to be short, a block does a whole one and writes the result.
 #include "attn_sm100.cuh"
 
 namespace ane_b200 {
@@ -27,27 +28,32 @@ constexpr uint32_t kMaxBatch = 1024;
 constexpr uint32_t kMaxBlocks = 512;   // of decode_kernel
 constexpr uint32_t kBigBlocks = 148;   // of prefix_kernel, about
 constexpr int kTile = 64;              // tokens per key/value tile
-constexpr int kThreads = 160;          // four computing warps and the producer
+constexpr int kThreads = 192;          // four computing warps, the producers of K and of V
 constexpr int kJoinThreads = 128;
 constexpr uint32_t kKept = 256;        // sequences whose slot and length stay in shared memory
-constexpr int kUnits = 2;              // units announced ahead
+constexpr int kPagesAhead = 4;         // tiles whose page numbers are read ahead
+constexpr int kUnits = 4;              // units announced ahead
 constexpr int kUnitCost = 2;           // a unit's start and end cost about what two tiles do
+constexpr uint32_t kWholeTiles = 10;   // units of at most so many tiles are not cut: 10 tiles take about
+                                       // what a second launch and the joining do
 
 struct Params {
     uint32_t batch, heads, kv_heads, group, dim, out_dtype;
     uint32_t shared;         // tokens of the prefix
     uint32_t prefix_tiles;   // its tiles in decode_kernel (0: none, or prefix_kernel does them)
-    uint32_t prefix_rts, own_rts;    // row tiles (16 rows) of a prefix / own unit
-    uint32_t prefix_rows, own_rows;  // rows of a partial result
+    uint32_t per_unit;       // sequences of a unit
+    uint32_t groups, subs;   // units per key/value head: groups of sequences x parts of 16 heads
+    uint32_t rows;           // rows of a unit's partial result
+    uint32_t whole;          // 1: a block per unit, results written
     uint32_t big_splits;     // spans of prefix_kernel (0: not used)
     uint32_t n_slots, max_pages, pages, page_shift, box_keys;
     float scale2;
     ane_rows q, out;
     const int32_t *tables, *lens, *slots;
     float* lse;
-    int32_t* cum;       // [batch + 1] steps of the own units of the sequences before b, per head; then steps per block
-    float *po, *pm;     // prefix partials: rows x dim; rows x {m, l}
-    float *so, *sm;     // the sequences' own
+    int32_t* cum;       // [batch + 1] own tiles of the sequences before b; then steps per block
+    float *po, *pm;     // prefix_kernel's partials: rows x dim; rows x {m, l}
+    float *so, *sm;     // decode_kernel's
     int* err;
 };
 
@@ -66,8 +72,27 @@ __device__ __forceinline__ int own_base(const Params& p) { return (int)(p.shared
 __device__ __forceinline__ int own_tiles(const Params& p, int len) {
     return len > (int)p.shared ? (len - own_base(p) + kTile - 1) / kTile : 0;
 }
-// Places of a unit of n tiles on the line that is cut into spans.
-__host__ __device__ __forceinline__ int steps(int tiles) { return tiles > 0 ? tiles + kUnitCost : 0; }
+// Place on the line where the units of group g begin, counted per head and part.
+// cum: own tiles of the sequences before b.
+__device__ __forceinline__ int group_start(const Params& p, const int32_t* cum, uint32_t g) {
+    return (int)(g * (kUnitCost + p.prefix_tiles)) + cum[min(g * p.per_unit, p.batch)];
+}
+// A unit's row: sequence (of the unit) and head (of its part of 16, or of the
+// group); the same for all units.
+struct RowPlace {
+    uint16_t seq, head;
+};
+__device__ __forceinline__ RowPlace row_place(const Params& p, uint32_t row) {
+    if (p.group > 16) return {0, (uint16_t)row};
+    return {(uint16_t)(row / p.group), (uint16_t)(row % p.group)};
+}
+// Sequence and head of the group; false: no such row.
+__device__ __forceinline__ bool row_of(const Params& p, uint32_t grp, uint32_t sub, RowPlace r, uint32_t& b,
+                                       uint32_t& g) {
+    b = grp * p.per_unit + r.seq;
+    g = sub * 16 + r.head;
+    return r.seq < p.per_unit && b < p.batch && g < p.group;
+}
 // {token in page, page} of key j; entries past the row and pages outside the
 // pool are never followed.
 __device__ __forceinline__ int2 page_of(const Params& p, const int32_t* table, int j) {
@@ -77,10 +102,13 @@ __device__ __forceinline__ int2 page_of(const Params& p, const int32_t* table, i
 }
 
 struct Unit {
-    int prefix, head, b, rt;  // b: sequence (own units); rt: row tile; head -1: no more units
-    int t0, t1;               // tiles
-    int base, lo, kend;       // key of tile 0; keys lo .. kend - 1 count
-    int slot;                 // place of the partial result
+    int head, grp, sub;  // head -1: no more units
+    int t0, t1;          // tiles
+    int slot;            // place of the partial result
+};
+struct Tile {
+    int who;             // sequence of the unit, -1: the prefix
+    int key, lo, kend;   // its first key; keys lo .. kend - 1 count
 };
 
 template <int DP>
@@ -89,13 +117,15 @@ struct DecodeSmem {
     static constexpr int kHalf = kTile * 128;        // 64 tokens x 64 elements
     static constexpr int kBytes = kTile * DP * 2;    // a K or a V tile
     uint8_t kv[kStages][2][kBytes];
-    uint8_t q[kUnits][16 * DP * 2];  // query rows of a unit
-    int vis[kUnits][16];             // keys that count for each row, from the unit's lo
+    uint8_t q[2][16 * DP * 2];       // query rows of this unit and the next
+    int vis[2][16];                  // prefix keys that each row sees
     float2 ml[kStages][4][16];       // {m, l} of each warp's rows
-    int cum[kMaxBatch + 1];          // steps of the own units of the sequences before b, per head
+    int cum[kMaxBatch + 1];          // own tiles of the sequences before b
     int2 seq[kKept];                 // {slot, len} of the first sequences
     Unit unit[kUnits];
-    uint64_t full[kStages], empty[kStages], joined[kStages], unit_full[kUnits], unit_empty[kUnits];
+    Tile tile[kStages];
+    RowPlace place[16];
+    uint64_t full[kStages], empty[kStages], joined[kStages], unit_full[kUnits], unit_empty[kUnits], q_full[2];
 };
 template <int DP>
 constexpr size_t decode_smem_bytes() {
@@ -122,7 +152,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t byt
 template <int DP>
 struct Query {
     uint32_t q[DP / 16][4];
-    int vis[2];
+    int vis[2];  // keys of the present tile's part that the row sees, from its lo
 };
 template <int DP>
 struct Sums {
@@ -212,9 +242,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x < 16) sm.place[threadIdx.x] = row_place(p, threadIdx.x);
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; s++) {
-            ptx::mbar_init(&sm.full[s], 1);
+            ptx::mbar_init(&sm.full[s], 2);
             ptx::mbar_init(&sm.empty[s], 4);
             ptx::mbar_init(&sm.joined[s], 4);
         }
@@ -222,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             ptx::mbar_init(&sm.unit_full[u], 1);
             ptx::mbar_init(&sm.unit_empty[u], 4);
         }
+        for (int q = 0; q < 2; q++) ptx::mbar_init(&sm.q_full[q], 129);  // all computing threads, and the row limits
         ptx::fence_mbarrier_init();
         ptx::prefetch_tmap(&map_k);
         ptx::prefetch_tmap(&map_v);
@@ -237,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) {
         const int2 q = seq_of(p, b);
         if (b < kKept) sm.seq[b] = q;
-        sm.cum[b] = steps(own_tiles(p, q.y));
+        sm.cum[b] = own_tiles(p, q.y);
     }
     auto seq = [&](uint32_t b) { return b < kKept ? sm.seq[b] : seq_of(p, b); };
     __syncthreads();
@@ -257,55 +289,48 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0) sm.cum[p.batch] = base;
     }
     __syncthreads();
-    const int prefix_steps = steps((int)p.prefix_tiles), prefix_all = prefix_steps * (int)(p.prefix_rts * p.kv_heads);
-    const int per_b = (int)(p.kv_heads * p.own_rts);  // own units of a sequence
-    const int total = prefix_all + sm.cum[p.batch] * per_b;
+    const int per_g = (int)(p.kv_heads * p.subs);  // units of a group
+    const int total = group_start(p, sm.cum, p.groups) * per_g;
     const int per = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
-    if (blockIdx.x == 0) {
+    if (blockIdx.x == 0 && !p.whole) {
         for (uint32_t b = threadIdx.x; b <= p.batch; b += kThreads) p.cum[b] = sm.cum[b];
         if (threadIdx.x == 0) p.cum[p.batch + 1] = per;
     }
-    const int64_t start = (int64_t)blockIdx.x * per;
 
-    if (warp == 4) {
-        // --------------------------------------------------------- producer
-        int at = (int)min(start, (int64_t)total);
-        const int end = (int)min(start + per, (int64_t)total);
-        int b_now = -1, len_now = 0;  // the sequence of the last own unit
+    if (warp >= 4) {
+        // -------------------------------------------------------- producers
+        // warp 4 loads K and announces units, warp 5 loads V
+        const bool is_v = warp == 5;
+        int at = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+        const int end = (int)min((int64_t)(blockIdx.x + 1) * per, (int64_t)total);
+        int g_now = 0;
+        bool done = false;
         auto next_unit = [&] {  // the unit with the next tile; moves `at` past its part of the span
             Unit u{};
             u.head = -1;
+            if (p.whole) {
+                if (done) return u;
+                done = true;
+                u.grp = (int)blockIdx.x / per_g;
+                const int id = (int)blockIdx.x % per_g;
+                u.head = id / (int)p.subs;
+                u.sub = id % (int)p.subs;
+                u.t1 = group_start(p, sm.cum, u.grp + 1) - group_start(p, sm.cum, u.grp) - kUnitCost;
+                return u;
+            }
             while (at < end) {
-                int first, n;
-                if (at < prefix_all) {
-                    const int id = at / prefix_steps;
-                    u.prefix = 1;
-                    u.head = id / (int)p.prefix_rts;
-                    u.rt = id % (int)p.prefix_rts;
-                    n = prefix_steps;
-                    first = id * n;
-                    u.slot = (int)blockIdx.x + id;
-                    u.kend = (int)p.shared;
-                } else {
-                    const int x = (at - prefix_all) / per_b;  // cum[b] <= x < cum[b + 1]
-                    int lo = max(b_now, 0), hi = (int)p.batch - 1;
-                    while (lo < hi) {
-                        const int mid = (lo + hi + 1) >> 1;
-                        if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1;
-                    }
-                    if (lo != b_now) len_now = seq((uint32_t)lo).y, b_now = lo;
-                    u.prefix = 0;
-                    u.b = lo;
-                    n = sm.cum[lo + 1] - sm.cum[lo];
-                    const int id = (at - prefix_all - sm.cum[lo] * per_b) / n;
-                    u.head = id / (int)p.own_rts;
-                    u.rt = id % (int)p.own_rts;
-                    first = prefix_all + sm.cum[lo] * per_b + id * n;
-                    u.slot = (int)blockIdx.x + lo * per_b + id;
-                    u.base = own_base(p);
-                    u.lo = (int)p.shared;
-                    u.kend = len_now;
+                const int x = at / per_g;  // start(g) <= x < start(g + 1)
+                int hi = (int)p.groups - 1;
+                while (g_now < hi) {
+                    const int mid = (g_now + hi + 1) >> 1;
+                    if (group_start(p, sm.cum, mid) <= x) g_now = mid; else hi = mid - 1;
                 }
+                const int g0 = group_start(p, sm.cum, g_now), n = group_start(p, sm.cum, g_now + 1) - g0;
+                const int id = (at - g0 * per_g) / n, first = g0 * per_g + id * n;
+                u.grp = g_now;
+                u.head = id / (int)p.subs;
+                u.sub = id % (int)p.subs;
+                u.slot = (int)blockIdx.x + g_now * per_g + id;
                 u.t0 = max(at - first - kUnitCost, 0);
                 u.t1 = min(n, end - first) - kUnitCost;
                 at = first + min(n, end - first);
@@ -316,102 +341,167 @@ __global__ void __launch_bounds__(kThreads, 2)
         };
         uint32_t said = 0, n = 0;
         bool ok = true;
-        // query rows of a unit on their way to its place, which has to be free
-        auto fetch_query = [&](const Unit& u) {
-            const uint32_t e = said % kUnits, rows = u.prefix ? p.batch * p.group : p.group;
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.unit_empty[e], ((said / kUnits) & 1) ^ 1, p.err));
-            if (!ok || u.head < 0) return;
-            constexpr int kChunks = DP / 8;
-#pragma unroll
-            for (int i = 0; i < 16 * kChunks / 32; i++) {
-                const uint32_t row = (uint32_t)(i * 32 + lane) / kChunks, ch = (uint32_t)lane % kChunks;
-                const uint32_t flat = (uint32_t)u.rt * 16 + row;
-                const bool on = flat < rows && ch * 8 < p.dim;
-                const uint32_t b = u.prefix ? flat / p.group : (uint32_t)u.b, g = u.prefix ? flat % p.group : flat;
-                const uint16_t* src = static_cast<const uint16_t*>(p.q.data) +
-                                      (on ? (size_t)b * p.q.token_stride + (size_t)(u.head * p.group + g) * p.q.head_stride + ch * 8 : 0);
-                cp16(ptx::smem_u32(sm.q[e] + q_off(row, ch)), src, on ? 16 : 0);
-            }
-            if (lane < 16) {
-                const uint32_t flat = (uint32_t)u.rt * 16 + lane;
-                sm.vis[e][lane] = flat >= rows ? 0 : u.prefix ? min(seq(flat / p.group).y, (int)p.shared) : u.kend - u.lo;
-            }
-        };
         auto announce = [&](const Unit& u) {
+            if (is_v) return;
             const uint32_t e = said % kUnits;
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
+            ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(&sm.unit_empty[e], ((said / kUnits) & 1) ^ 1, p.err));
+            if (ok && lane == 0) {
                 sm.unit[e] = u;
                 ptx::mbar_arrive(&sm.unit_full[e]);
             }
             said++;
         };
-        // one lane per box: K or V, 64 elements, box_keys tokens
+        // one lane per box: 64 elements, box_keys tokens
         constexpr int kHalves = DP / 64;
-        const int key_boxes = kTile / (int)p.box_keys, boxes = key_boxes * kHalves;
-        const bool is_v = lane >= boxes, lane_on = lane < 2 * boxes;
-        const int box = is_v ? lane - boxes : lane;
-        const int key0 = box / kHalves * (int)p.box_keys, half = box % kHalves;
-        auto table_of = [&](const Unit& x) {
-            return p.tables + (size_t)max(seq(x.prefix ? 0 : (uint32_t)x.b).x, 0) * p.max_pages;
+        const int box_shift = 31 - __clz((int)p.box_keys), key_boxes = kTile >> box_shift, boxes = key_boxes * kHalves;
+        const bool lane_on = lane < boxes;
+        const int key0 = lane / kHalves * (int)p.box_keys, half = lane % kHalves;
+        const CUtensorMap* map = is_v ? &map_v : &map_k;
+        // Where tiles come from: a tile, its sequence's table, tiles left of that.
+        struct Cursor {
+            Tile t;
+            const int32_t* table;
+            int left;
         };
-        auto entry = [&](const int32_t* table, int j, int kend) {  // page number of this lane's box
-            return lane_on && j < kend ? __ldcg(table + min((uint32_t)j >> p.page_shift, p.max_pages - 1)) : 0;
+        auto own = [&](int b) { return sm.cum[b + 1] - sm.cum[b]; };
+        auto to_sequence = [&](Cursor& c, const Unit& u, int b, int skip) {
+            const int2 q = seq((uint32_t)b);
+            c.t = Tile{b - u.grp * (int)p.per_unit, own_base(p) + skip * kTile, (int)p.shared, q.y};
+            c.table = p.tables + (size_t)max(q.x, 0) * p.max_pages;
+            c.left = own(b) - skip;
         };
-        Unit u = next_unit();
-        const int32_t* table = u.head >= 0 ? table_of(u) : p.tables;
-        int page = u.head >= 0 ? entry(table, u.base + u.t0 * kTile + key0, u.kend) : 0;
-        fetch_query(u);
-        if (ok) announce(u);
-        while (ok && u.head >= 0) {
-            // what the next unit starts with is read while this one loads
-            const Unit following = next_unit();
-            const bool more = following.head >= 0;
-            const int32_t* table_f =
-                !more ? table : following.prefix == u.prefix && following.b == u.b ? table : table_of(following);
-            const int page_f = more ? entry(table_f, following.base + following.t0 * kTile + key0, following.kend) : 0;
-            fetch_query(following);
-            int j = u.base + u.t0 * kTile + key0;
-            for (int t = u.t0; t < u.t1 && ok; t++, j += kTile, n++) {
-                const int page_n = t + 1 < u.t1 ? entry(table, j + kTile, u.kend) : 0;
-                const uint32_t st = n % S::kStages;
-                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.empty[st], ((n / S::kStages) & 1) ^ 1, p.err));
-                if (!ok) break;
-                // boxes past the last key are left out
-                const int live = min(key_boxes, (u.kend - (u.base + t * kTile) + (int)p.box_keys - 1) / (int)p.box_keys);
-                if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.full[st], 2 * kHalves * 128 * p.box_keys * live);
-                __syncwarp();
-                if (lane_on && j < u.kend)
-                    tma_load_4d(sm.kv[st][is_v] + half * S::kHalf + key0 * 128, is_v ? &map_v : &map_k, &sm.full[st],
-                                half * 64, u.head, j & ((1 << p.page_shift) - 1), (uint32_t)page < p.pages ? page : 0);
-                page = page_n;
+        auto seek = [&](const Unit& u) {  // u has tiles
+            Cursor c;
+            int t = u.t0, b = u.grp * (int)p.per_unit;
+            if (t < (int)p.prefix_tiles) {
+                c.t = Tile{-1, t * kTile, 0, (int)p.shared};
+                c.table = p.tables + (size_t)max(seq(0).x, 0) * p.max_pages;
+                c.left = (int)p.prefix_tiles - t;
+                return c;
             }
-            if (!ok) break;
+            t -= (int)p.prefix_tiles;
+            while (t >= own(b)) t -= own(b++);
+            to_sequence(c, u, b, t);
+            return c;
+        };
+        auto advance = [&](Cursor& c, const Unit& u) {  // there is a next tile
+            c.t.key += kTile;
+            if (--c.left) return;
+            int b = u.grp * (int)p.per_unit + c.t.who + 1;
+            while (own(b) == 0) b++;
+            to_sequence(c, u, b, 0);
+        };
+        auto entry = [&](const Cursor& c) {  // page number of this lane's box
+            const int j = c.t.key + key0;
+            return lane_on && j < c.t.kend ? __ldcg(c.table + min((uint32_t)j >> p.page_shift, p.max_pages - 1)) : 0;
+        };
+        // A unit's cursors (tile to load; tile whose page is read) and the page
+        // numbers between them.
+        struct Ahead {
+            Cursor load, read;
+            int page[kPagesAhead];
+        };
+        auto begin = [&](const Unit& u) {  // u has tiles
+            Ahead a;
+            a.load = a.read = seek(u);
+#pragma unroll
+            for (int d = 0; d < kPagesAhead; d++) {
+                a.page[d] = 0;
+                if (u.t0 + d >= u.t1) continue;
+                if (d) advance(a.read, u);
+                a.page[d] = entry(a.read);
+            }
+            return a;
+        };
+        Unit u = next_unit(), following = u;
+        announce(u);
+        Ahead a{}, af{};
+        if (u.head >= 0 && u.t1 > u.t0) a = begin(u);
+        // announces the next unit and reads what it starts with
+        auto look_ahead = [&] {
+            following = next_unit();
             announce(following);
+            if (following.head >= 0) af = begin(following);
+        };
+        while (ok && u.head >= 0) {
+            if (u.t1 <= u.t0) look_ahead();
+            int t = u.t0;
+            while (ok && t < u.t1) {
+#pragma unroll
+                for (int d = 0; d < kPagesAhead; d++) {  // (page numbers on their way cannot change registers)
+                    if (!ok || t >= u.t1) continue;
+                    const Tile now = a.load.t;
+                    const int page = a.page[d];
+                    if (t + 1 < u.t1) advance(a.load, u);
+                    const uint32_t st = n % S::kStages;
+                    ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.empty[st], ((n / S::kStages) & 1) ^ 1, p.err));
+                    if (!ok) continue;
+                    // boxes past the last key are left out
+                    const int live = min(key_boxes, (now.kend - now.key + (int)p.box_keys - 1) >> box_shift);
+                    if (lane == 0) {
+                        if (!is_v) sm.tile[st] = now;
+                        ptx::mbar_arrive_expect_tx(&sm.full[st], kHalves * 128 * p.box_keys * live);
+                    }
+                    __syncwarp();
+                    const int j = now.key + key0;
+                    if (lane_on && j < now.kend)
+                        tma_load_4d(sm.kv[st][is_v] + half * S::kHalf + key0 * 128, map, &sm.full[st],
+                                    half * 64, u.head, j & ((1 << p.page_shift) - 1), (uint32_t)page < p.pages ? page : 0);
+                    if (t + kPagesAhead < u.t1) advance(a.read, u), a.page[d] = entry(a.read);
+                    // with the first tiles on their way
+                    if (t == min(u.t0 + S::kStages, u.t1) - 1) look_ahead();
+                    t++;
+                    n++;
+                }
+            }
             u = following;
-            table = table_f;
-            page = page_f;
+            a = af;
         }
     } else {
         // -------------------------------------------------------- computing
         uint32_t seen = 0, n = 0, join_phase = 0;
         bool ok = true;
-        while (true) {
-            const uint32_t e = seen % kUnits;
+        const RowPlace place[2] = {sm.place[lane / 4], sm.place[lane / 4 + 8]};
+        Unit u, un;
+        // the next unit, and its query rows on their way to the other place
+        auto fetch = [&](Unit& dst) {
+            const uint32_t e = seen % kUnits, to = seen & 1;
             ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.unit_full[e], (seen / kUnits) & 1, p.err));
-            if (!ok) break;
+            if (!ok) return;
             seen++;
-            const Unit u = sm.unit[e];
-            if (u.head < 0) break;
+            dst = sm.unit[e];
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&sm.unit_empty[e]);
+            if (dst.head < 0) return;
+            constexpr int kChunks = DP / 8;
+            uint32_t b, g;
+#pragma unroll
+            for (int i = 0; i < kChunks / 8; i++) {
+                const uint32_t c = threadIdx.x + i * 128, row = c / kChunks, ch = c % kChunks;
+                const bool on = row_of(p, dst.grp, dst.sub, sm.place[row], b, g) && ch * 8 < p.dim;
+                const uint16_t* src = static_cast<const uint16_t*>(p.q.data) +
+                                      (on ? (size_t)b * p.q.token_stride + (size_t)(dst.head * p.group + g) * p.q.head_stride + ch * 8 : 0);
+                cp16(ptx::smem_u32(sm.q[to] + q_off(row, ch)), src, on ? 16 : 0);
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(&sm.q_full[to])) : "memory");
+            if (warp == 0) {
+                if (lane < 16)
+                    sm.vis[to][lane] = row_of(p, dst.grp, dst.sub, sm.place[lane], b, g) ? min(seq(b).y, (int)p.shared) : 0;
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&sm.q_full[to]);
+            }
+        };
+        fetch(u);
+        for (uint32_t nu = 0; ok && u.head >= 0; nu++, u = un) {
+            const uint32_t e = nu & 1;
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.q_full[e], (nu >> 1) & 1, p.err));
+            if (!ok) break;
             Query<DP> q;
 #pragma unroll
             for (int kk = 0; kk < DP / 16; kk++)
                 ldsm4(ptx::smem_u32(sm.q[e] + q_off((lane >> 3 & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4))), q.q[kk]);
-            q.vis[0] = sm.vis[e][lane / 4];
-            q.vis[1] = sm.vis[e][lane / 4 + 8];
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sm.unit_empty[e]);
+            const int vis[2] = {sm.vis[e][lane / 4], sm.vis[e][lane / 4 + 8]};
+            un.head = -2;  // not looked at yet
             Sums<DP> r;
 #pragma unroll
             for (int i = 0; i < DP / 8; i++) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
@@ -422,23 +512,28 @@ __global__ void __launch_bounds__(kThreads, 2)
                 st = n % S::kStages;
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.full[st], (n / S::kStages) & 1, p.err));
                 if (!ok) break;
-                const int j0 = u.base + t * kTile + warp * 16;
-                if (j0 + 16 > u.kend || j0 < u.lo) {
+                const Tile now = sm.tile[st];
+                const int j0 = now.key + warp * 16;
+                if (j0 + 16 > now.kend || j0 < now.lo) {
                     // rows of V that do not count: a weight of 0 does not silence a NaN
                     for (int i = lane; i < 16 * DP / 8; i += 32) {
-                        const int tok = warp * 16 + i % 16;
-                        const int key = u.base + t * kTile + tok;
-                        if (key >= u.kend || key < u.lo)
+                        const int tok = warp * 16 + i % 16, key = now.key + tok;
+                        if (key >= now.kend || key < now.lo)
                             *reinterpret_cast<uint4*>(sm.kv[st][1] + tile_off(tok, i / 16)) = make_uint4(0, 0, 0, 0);
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                 }
-                if (j0 < u.kend && j0 + 16 > u.lo)
+                if (j0 < now.kend && j0 + 16 > now.lo) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) q.vis[h] = now.who < 0 ? vis[h] : (int)place[h].seq == now.who ? now.kend - now.lo : 0;
                     tile_step<T, DP>(q, r, ptx::smem_u32(sm.kv[st][0]), ptx::smem_u32(sm.kv[st][1]), warp * 16,
-                                     j0 - u.lo, p.scale2);
+                                     j0 - now.lo, p.scale2);
+                }
                 __syncwarp();
                 if (t + 1 < u.t1 && lane == 0) ptx::mbar_arrive(&sm.empty[st]);
+                if (t == u.t0) fetch(un);
+                if (!ok) break;
             }
             if (!ok) break;
 #pragma unroll
@@ -446,60 +541,77 @@ __global__ void __launch_bounds__(kThreads, 2)
                 r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 1);
                 r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 2);
             }
-            // the warps' sums meet in the last tile's stage, which is still theirs;
-            // each warp joins a quarter of the columns
             constexpr int kQuarter = DP / 8;  // words per lane
-            if ((lane & 3) == 0) {
-                sm.ml[st][warp][lane / 4] = make_float2(r.m[0], r.l[0]);
-                sm.ml[st][warp][lane / 4 + 8] = make_float2(r.m[1], r.l[1]);
-            }
-#pragma unroll
-            for (int i = 0; i < DP / 2; i++) *spill<DP>(sm.kv[st], warp, i) = r.o[i >> 2][i & 3];
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sm.joined[st]);
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.joined[st], (join_phase >> st) & 1, p.err));
-            if (!ok) break;
-            join_phase ^= 1u << st;
             float m[2] = {kNegInf, kNegInf}, l[2] = {0.0f, 0.0f}, o[kQuarter];
-            float2 ml[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    ml[h][w] = sm.ml[st][w][lane / 4 + 8 * h];
-                    m[h] = fmaxf(m[h], ml[h][w].x);
-                }
 #pragma unroll
             for (int i = 0; i < kQuarter; i++) o[i] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                float f[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    f[h] = exp2_fast(ml[h][w].x - (m[h] == kNegInf ? 0.0f : m[h]));
-                    l[h] += ml[h][w].y * f[h];
+            if (u.t1 <= u.t0) fetch(un);
+            if (!ok) break;
+            if (u.t1 > u.t0) {
+                // the warps' sums meet in the last tile's stage, which is still theirs;
+                // each warp joins a quarter of the columns
+                if ((lane & 3) == 0) {
+                    sm.ml[st][warp][lane / 4] = make_float2(r.m[0], r.l[0]);
+                    sm.ml[st][warp][lane / 4 + 8] = make_float2(r.m[1], r.l[1]);
                 }
 #pragma unroll
-                for (int i = 0; i < kQuarter; i++) o[i] += *spill<DP>(sm.kv[st], w, warp * kQuarter + i) * f[(i & 3) >> 1];
+                for (int i = 0; i < DP / 2; i++) *spill<DP>(sm.kv[st], warp, i) = r.o[i >> 2][i & 3];
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&sm.joined[st]);
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.joined[st], (join_phase >> st) & 1, p.err));
+                if (!ok) break;
+                join_phase ^= 1u << st;
+                float2 ml[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        ml[h][w] = sm.ml[st][w][lane / 4 + 8 * h];
+                        m[h] = fmaxf(m[h], ml[h][w].x);
+                    }
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    float f[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        f[h] = exp2_fast(ml[h][w].x - (m[h] == kNegInf ? 0.0f : m[h]));
+                        l[h] += ml[h][w].y * f[h];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kQuarter; i++) o[i] += *spill<DP>(sm.kv[st], w, warp * kQuarter + i) * f[(i & 3) >> 1];
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&sm.empty[st]);
             }
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sm.empty[st]);
-            float* po = u.prefix ? p.po : p.so;
-            float* pml = u.prefix ? p.pm : p.sm;
-            const int rows = (int)(u.prefix ? p.prefix_rows : p.own_rows);
-            const int limit = min(rows, (int)(u.prefix ? p.batch * p.group : p.group) - u.rt * 16);
+            // rows of this warp's quarter of the columns
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int row = lane / 4 + 8 * h;
-                if (row >= limit) continue;
-                const size_t at = (size_t)u.slot * rows + row;
-                if (warp == 0 && (lane & 3) == 0) *reinterpret_cast<float2*>(pml + at * 2) = make_float2(m[h], l[h]);
+                const uint32_t row = lane / 4 + 8 * h;
+                uint32_t b, g;
+                if (!row_of(p, u.grp, u.sub, place[h], b, g)) continue;
+                const uint32_t head = u.head * p.group + g;
+                const bool empty = l[h] == 0.0f;
+                const float f = empty ? 0.0f : 1.0f / l[h];
+                const size_t at = (size_t)u.slot * p.rows + row;
+                uint8_t* out = static_cast<uint8_t*>(p.out.data) +
+                               ((size_t)b * p.out.token_stride + (size_t)head * p.out.head_stride) *
+                                   (p.out_dtype == ANE_DTYPE_F32 ? 4 : 2);
+                if (warp == 0 && (lane & 3) == 0) {
+                    if (!p.whole)
+                        *reinterpret_cast<float2*>(p.sm + at * 2) = make_float2(m[h], l[h]);
+                    else if (p.lse)
+                        p.lse[(size_t)b * p.heads + head] = empty ? kNegInf : (m[h] + log2f(l[h]) - Type<T>::kShift) * kLn2;
+                }
 #pragma unroll
                 for (int x = 0; x < kQuarter / 4; x++) {
                     const uint32_t c = (warp * (kQuarter / 4) + x) * 8 + 2 * (lane & 3);
-                    if (c < p.dim)
-                        *reinterpret_cast<float2*>(po + at * p.dim + c) = make_float2(o[4 * x + 2 * h], o[4 * x + 2 * h + 1]);
+                    if (c >= p.dim) continue;
+                    const float y0 = o[4 * x + 2 * h], y1 = o[4 * x + 2 * h + 1];
+                    if (!p.whole)
+                        *reinterpret_cast<float2*>(p.so + at * p.dim + c) = make_float2(y0, y1);
+                    else
+                        store2(out, c, p.out_dtype, empty ? 0.0f : y0 * f, empty ? 0.0f : y1 * f);
                 }
             }
         }
@@ -571,31 +683,23 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     ptx::griddep_wait();
     const uint32_t b = blockIdx.x, head = blockIdx.y, h = head / p.group, g = head % p.group;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = __ldcg(p.cum + p.batch + 1), c0 = __ldcg(p.cum + b), n = __ldcg(p.cum + b + 1) - c0;
-    // spans [pc, pe) and [oc, oe) of blocks hold partials of this row: of span c
-    // at row prow + c * pstep, orow + c * ostep
-    int pc = 0, pe = 0, oc = 0, oe = 0;
-    size_t prow = 0, pstep = 0;
-    const uint32_t flat = b * p.group + g;
-    if (p.big_splits) {
-        pe = (int)p.big_splits;
-        const size_t rows = (size_t)p.batch * p.group;
-        prow = (size_t)h * rows + flat;
-        pstep = rows * p.kv_heads;
-    } else if (p.prefix_tiles) {
-        const int id = (int)(h * p.prefix_rts + flat / 16), first = id * steps((int)p.prefix_tiles);
-        pc = (first + kUnitCost) / per;
-        pe = (first + steps((int)p.prefix_tiles) - 1) / per + 1;
-        prow = (size_t)id * p.prefix_rows + flat % 16;
-        pstep = p.prefix_rows;
-    }
-    const int per_b = (int)(p.kv_heads * p.own_rts), id = (int)(h * p.own_rts + g / 16);
-    const size_t orow = (size_t)((int)b * per_b + id) * p.own_rows + g % 16, ostep = p.own_rows;
+    // spans [pc, pe) of prefix_kernel and [oc, oe) of decode_kernel's blocks hold
+    // partials of this row: of span c at row prow + c * pstep, orow + c * p.rows
+    const int pc = 0, pe = (int)p.big_splits;
+    const size_t all_rows = (size_t)p.batch * p.group;
+    const size_t prow = (size_t)h * all_rows + b * p.group + g, pstep = all_rows * p.kv_heads;
+    const uint32_t grp = b / p.per_unit, sub = p.group > 16 ? g / 16 : 0;
+    const uint32_t row = p.group > 16 ? g % 16 : b % p.per_unit * p.group + g;
+    const int per = __ldcg(p.cum + p.batch + 1), per_g = (int)(p.kv_heads * p.subs), id = (int)(h * p.subs + sub);
+    const int c0 = __ldcg(p.cum + min(grp * p.per_unit, p.batch)), c1 = __ldcg(p.cum + min((grp + 1) * p.per_unit, p.batch));
+    const int n = c1 - c0 + (int)p.prefix_tiles;  // tiles of the row's unit
+    int oc = 0, oe = 0;
     if (n) {
-        const int first = steps((int)p.prefix_tiles) * (int)(p.prefix_rts * p.kv_heads) + c0 * per_b + id * n;
-        oc = (first + kUnitCost) / per;
+        const int first = ((int)(grp * (kUnitCost + p.prefix_tiles)) + c0) * per_g + id * (n + kUnitCost) + kUnitCost;
+        oc = first / per;
         oe = (first + n - 1) / per + 1;
     }
+    const size_t orow = (size_t)((int)grp * per_g + id) * p.rows + row;
     float m = kNegInf, l = 0.0f;
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool on = (uint32_t)lane * 4 < p.dim;
@@ -608,7 +712,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
         for (int k = 0; k < 4; k++) {
             const int i = i0 + 4 * k;
             const bool pre = i < pe - pc;
-            const size_t at = pre ? prow + (size_t)(pc + i) * pstep : orow + (size_t)(oc + i - (pe - pc)) * ostep;
+            const size_t at = pre ? prow + (size_t)(pc + i) * pstep : orow + (size_t)(oc + i - (pe - pc)) * p.rows;
             x[k] = make_float2(kNegInf, 0.0f);
             v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (i < count) {
@@ -655,24 +759,21 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
 
 // ------------------------------------------------------------------ launch
 struct Layout {
-    uint32_t prefix_rts, own_rts, prefix_rows, own_rows, pairs, big_splits;
+    uint32_t per_unit, groups, subs, rows, pairs, big_splits;
     size_t cum, pm, po, sm, so, bytes;
 };
 Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
     Layout l;
     const uint32_t group = heads / kv_heads;
-    const size_t rows = (size_t)batch * group;
-    l.prefix_rts = (uint32_t)ceil_div(rows, 16);
-    l.own_rts = (uint32_t)ceil_div(group, 16);
-    l.prefix_rows = (uint32_t)(rows < 16 ? rows : 16);
-    l.own_rows = group < 16 ? group : 16;
+    l.per_unit = group > 16 ? 1 : 16 / group;
+    l.groups = (uint32_t)ceil_div(batch, l.per_unit);
+    l.subs = (uint32_t)ceil_div(group, 16);
+    l.rows = group > 16 ? 16 : (l.per_unit < batch ? l.per_unit : batch) * group;
     l.pairs = (uint32_t)ceil_div(batch, 2 * (kBigRows / group));
     l.big_splits = kBigBlocks / (kv_heads * l.pairs);
     if (l.big_splits == 0) l.big_splits = 1;
-    const size_t prefix_small = (kMaxBlocks + (size_t)kv_heads * l.prefix_rts) * l.prefix_rows;
-    const size_t prefix_big = (size_t)l.big_splits * kv_heads * rows;
-    const size_t prefix_rows = prefix_small > prefix_big ? prefix_small : prefix_big;
-    const size_t own_rows = (kMaxBlocks + (size_t)batch * kv_heads * l.own_rts) * l.own_rows;
+    const size_t own_rows = (kMaxBlocks + (size_t)kv_heads * l.groups * l.subs) * l.rows;
+    const size_t prefix_rows = (size_t)l.big_splits * kv_heads * batch * group;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -701,8 +802,10 @@ int launch(const CUtensorMap (&map)[3], const Params& p, uint32_t pairs, cudaStr
             return rc;
     }
     if ((rc = set_max_dynamic_smem(decode_kernel<T, DP>, (int)decode_smem_bytes<DP>(), done))) return rc;
-    const uint32_t blocks = (uint32_t)num_sms() * 2 < kMaxBlocks ? (uint32_t)num_sms() * 2 : kMaxBlocks;
-    if ((rc = launch_pdl(decode_kernel<T, DP>, dim3(blocks), dim3(kThreads), decode_smem_bytes<DP>(), s, map[1], map[2], p)))
+    const uint32_t spans = (uint32_t)num_sms() * 2 < kMaxBlocks ? (uint32_t)num_sms() * 2 : kMaxBlocks;
+    const uint32_t blocks = p.whole ? p.kv_heads * p.groups * p.subs : spans;
+    if ((rc = launch_pdl(decode_kernel<T, DP>, dim3(blocks), dim3(kThreads), decode_smem_bytes<DP>(), s, map[1], map[2], p)) ||
+        p.whole)
         return rc;
     return launch_pdl(join_kernel<T>, dim3(p.batch, p.heads), dim3(kJoinThreads), 0, s, p);
 }
@@ -742,7 +845,7 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     const Layout l = layout(batch, heads, kv_heads, dim);
     const uint64_t most = (uint64_t)max_pages * pt;  // tokens of a slot
     ANE_ARG_CHECK(most <= 0x7fffff00u &&
-                      (most / kTile + 3) * kv_heads * ((uint64_t)batch * l.own_rts + l.prefix_rts) <= 0x7fffffffu,
+                      (most / kTile + kUnitCost + 2) * kv_heads * l.subs * ((uint64_t)batch + l.groups) <= 0x7fffffffu,
                   "attn_decode: more than 2^31 tiles of 64 tokens");
     ANE_ARG_CHECK(shared <= most, "attn_decode: shared exceeds max_pages pages");
     ANE_ARG_CHECK(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= l.bytes,
@@ -753,12 +856,13 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.batch = batch, p.heads = heads, p.kv_heads = kv_heads, p.group = heads / kv_heads, p.dim = dim;
     p.out_dtype = out_dtype;
     p.shared = shared;
-    // decode_kernel goes over the prefix once per 16 rows.  The second time costs
+    // decode_kernel goes over the prefix once per unit of 16 rows.  The second time costs
     // little (L2), every further one a tile's time: prefix_kernel from where that
     // makes eight tiles a block.  128 rows x 8 heads, 4096 shared: 31 us without it,
     // 25 with it; 1024 shared: 23 and 23; 64 rows x 32 heads, 1024 shared: 41 and 44;
     // 32 rows x 32 heads, 16384 shared: 74 and 86.
-    const uint64_t again = l.prefix_rts > 2 ? (uint64_t)(l.prefix_rts - 2) * kv_heads * ceil_div(shared, kTile) : 0;
+    const uint32_t units = l.groups * l.subs;
+    const uint64_t again = units > 2 ? (uint64_t)(units - 2) * kv_heads * ceil_div(shared, kTile) : 0;
     const bool big = again >= 8 * 2 * (uint64_t)kBigBlocks;
     if (big) {
         const uint32_t tiles = (uint32_t)ceil_div(shared, kBigKeys);
@@ -766,7 +870,7 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     } else {
         p.prefix_tiles = (uint32_t)ceil_div(shared, kTile);
     }
-    p.prefix_rts = l.prefix_rts, p.own_rts = l.own_rts, p.prefix_rows = l.prefix_rows, p.own_rows = l.own_rows;
+    p.per_unit = l.per_unit, p.groups = l.groups, p.subs = l.subs, p.rows = l.rows;
     p.n_slots = n_slots, p.max_pages = max_pages, p.pages = pages->pages;
     while ((1u << p.page_shift) < pt) p.page_shift++;
     p.scale2 = scale * attn::kLog2e;
@@ -778,6 +882,8 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.err = device_timeout_flag();
     // one box shape for both kernels: a page, or 64 tokens of a larger one
     p.box_keys = pt < (uint32_t)kTile ? pt : (uint32_t)kTile;
+    const uint64_t own = ceil_div(most - (shared & ~(p.box_keys - 1)), kTile);  // of a sequence, at most
+    p.whole = !big && p.prefix_tiles + (batch < l.per_unit ? batch : l.per_unit) * own <= kWholeTiles;
     const auto type = dtype == ANE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     CUtensorMap map[3];
     if (big && (rc = encode_tensor_map_3d(&map[0], type, q->data, {dim, heads, batch},
