@@ -16,11 +16,17 @@
 //
 // What bounds it: per tile of 128 x 128 scores and head dim 128 the tensor cores
 // take 1024 cycles (both products), the 16384 exponentials 1024 cycles of the
-// special-function unit, and each tile's products wait for its exponentials.  So
-// P is handed over in parts while the rest is computed, and a tile's first
-// weights do not wait for its maximum.  (Some of the exponentials as a polynomial
-// on the FMA units was slower, 16384 tokens: 0, 2, 3, 4 of eight 1613, 1791, 1790,
-// 1899 us.)
+// special-function units, and a tile's products wait for its exponentials, the
+// next scores for those products.  Measured per pair of tiles: 2800 cycles at head
+// dim 64 and 128 alike, 73 % of the tensor cores' time at 128; a tile on its own
+// takes as long, so it is that chain (scores ready -> weights 2500 cycles -> last
+// products and next scores 960) that is left.  Hence P is handed over in parts and
+// the weights do not wait for the tile's maximum.  Tried and slower (16384 tokens,
+// 1613 us then): 2, 3, 4 of eight exponentials as a polynomial on the FMA units
+// (1791, 1790, 1899); two threads per row (2250); the two warps of a scheduler
+// taking turns at their exponentials (1635); with head dim 64, P apart from S so
+// that the next scores do not wait for P (174 -> 190 us on a block of 1024).  Over
+// seconds the chip's power limit holds the clock at 1.45 GHz.
 //
 // Warps (384 threads): 0-3 and 4-7 softmax of tile 0 and 1; 8 loads (TMA);
 // 9 issues the MMAs and owns TMEM; 10 clears the rows of V that lie past the
@@ -464,11 +470,18 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                     if (lane == 0) ptx::mbar_arrive(&sm.p_part[part][t]);
                 };
                 const int rest = vis - j * kBigKeys;  // keys of this tile that the row sees
-                float top;
+                // P goes out while the next keys' weights are computed
+                auto first_three = [&](bool have) {
+                    if (!have) weights(0);
+                    ptx::tmem_st_32x32b_x16(ts, w);
+                    weights(1);
+                    ptx::tmem_st_32x32b_x16(ts + 16, w);
+                    weights(2);
+                };
                 if (j > begin && __all_sync(0xffffffffu, rest >= kBigKeys)) {
                     // The reference of the tiles before will do for this one too,
-                    // nearly always: its first weights are under way before the
-                    // tile's maximum is known.
+                    // nearly always: the weights do not wait for the tile's maximum,
+                    // which is looked at before any of them is handed over.
                     ptx::tmem_ld_32x32b_x32(ts, s[0]);
                     ptx::tmem_ld_wait();
                     ptx::pin32(s[0]);
@@ -478,10 +491,11 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int c = 1; c < 4; c++) ptx::pin32(s[c]);
-                    top = largest();
+                    first_three(true);
+                    const float top = largest();
                     if (__any_sync(0xffffffffu, top > m + kSlack)) {
                         raise(top);
-                        weights(0);
+                        first_three(false);
                     }
                 } else {
 #pragma unroll
@@ -494,15 +508,10 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                     for (int c = 0; c < 4; c++)
 #pragma unroll
                         for (int x = 0; x < 32; x++) s[c][x] = c * 32 + x < rest ? s[c][x] : 0xff800000u;
-                    top = largest();
+                    const float top = largest();
                     if (__any_sync(0xffffffffu, top > m + kSlack)) raise(top);
-                    weights(0);
+                    first_three(false);
                 }
-                // P goes out while the next keys' weights are computed
-                ptx::tmem_st_32x32b_x16(ts, w);
-                weights(1);
-                ptx::tmem_st_32x32b_x16(ts + 16, w);
-                weights(2);
                 arrive(0);
                 ptx::tmem_st_32x32b_x16(ts + 32, w);
                 weights(3);
