@@ -224,6 +224,51 @@ __device__ __forceinline__ void tile_step(const Query<DP>& q, Sums<DP>& r, uint3
     }
 }
 
+// A unit's rows belong to several sequences, and the product of a weight of 0 with
+// an infinity or NaN in another sequence's V would reach them.  So such values of
+// a sequence's own V (16 tokens of a tile; nothing is there but in a broken cache)
+// go to that sequence's rows by themselves and are cleared before the products.
+// One warp; tok0: its first token row, `sees`: whether the thread's rows see it.
+template <typename T, int DP>
+__device__ __forceinline__ void set_apart(Sums<DP>& r, uint8_t* v, uint32_t tok0, const bool (&sees)[2]) {
+    constexpr uint32_t kLimit = sizeof(T) && Type<T>::kShift > 0.0f ? 0x7c00u : 0x7f80u;  // infinity
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t most = 0;  // the largest magnitudes, as integers, in the two halves
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) {
+        const uint32_t e = i * 32 + lane;
+        const uint4 x = *reinterpret_cast<const uint4*>(v + tile_off(tok0 + e % 16, e / 16));
+        most = __vmaxu2(__vmaxu2(most, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+        most = __vmaxu2(__vmaxu2(most, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
+    }
+    if (!__any_sync(0xffffffffu, (most & 0xffffu) >= kLimit || (most >> 16) >= kLimit)) return;
+    for (uint32_t t = 0; t < 16; t++) {
+#pragma unroll
+        for (int x = 0; x < DP / 8; x++) {
+            const uint32_t two = *reinterpret_cast<const uint32_t*>(v + tile_off(tok0 + t, x) + 4 * (lane & 3));
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint16_t bits = (uint16_t)(two >> (16 * k));
+                if ((bits & 0x7fffu) < kLimit) continue;
+                const float f = (bits & 0x7fffu) > kLimit ? NAN : (bits >> 15) ? -INFINITY : INFINITY;
+                if (sees[0]) r.o[x][k] += f;
+                if (sees[1]) r.o[x][2 + k] += f;
+            }
+        }
+    }
+    __syncwarp();
+    for (int i = 0; i < DP / 16; i++) {
+        const uint32_t e = i * 32 + lane;
+        uint32_t* x = reinterpret_cast<uint32_t*>(v + tile_off(tok0 + e % 16, e / 16));
+        for (int k = 0; k < 4; k++) {
+            if ((x[k] & 0x7fffu) >= kLimit) x[k] &= 0xffff0000u;
+            if ((x[k] >> 16 & 0x7fffu) >= kLimit) x[k] &= 0x0000ffffu;
+        }
+    }
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+}
+
 // Word i of this lane's accumulators in the 16 token rows of a stage that only
 // `warp` reads (and has read).  Words 4 x .. 4 x + 3 are column block x of 8.
 template <int DP>
@@ -527,6 +572,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (j0 < now.kend && j0 + 16 > now.lo) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) q.vis[h] = now.who < 0 ? vis[h] : (int)place[h].seq == now.who ? now.kend - now.lo : 0;
+                    if (now.who >= 0 && p.per_unit > 1 && p.batch > 1)
+                        set_apart<T, DP>(r, sm.kv[st][1], warp * 16, {q.vis[0] > 0, q.vis[1] > 0});
                     tile_step<T, DP>(q, r, ptx::smem_u32(sm.kv[st][0]), ptx::smem_u32(sm.kv[st][1]), warp * 16,
                                      j0 - now.lo, p.scale2);
                 }

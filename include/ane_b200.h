@@ -456,10 +456,11 @@ typedef struct ane_rows {
  * Query head h reads key/value head h / (heads / kv_heads):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][hk]) * v[j][hk]
  * A query that sees no key (lk < lq) gives 0 (and lse -inf).  Rows outside the
- * sequence are never part of a result, whatever they hold.  lse (NULL to skip)
+ * sequence are never part of a result, whatever they hold; inside it v has to be
+ * finite (a key that a query does not see yet has weight 0, and 0 * NaN is NaN).  lse (NULL to skip)
  * receives [total_q][heads] natural logarithms of the softmax sums.
- * dim % 8 == 0, dim <= 128; heads a multiple of kv_heads, at most 64 per
- * kv_head; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold.
+ * scale > 0; dim % 8 == 0, dim <= 128; heads a multiple of kv_heads, at most 64
+ * per kv_head; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold.
  * workspace: 256-byte aligned, ane_attn_prompt_workspace_size bytes (which may be
  * 0), any contents, not shared by calls that may overlap. */
 size_t ane_attn_prompt_workspace_size(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t dim,
@@ -484,13 +485,15 @@ typedef struct ane_pages {
  * Row b of q / out belongs to slot slots[b] (NULL: b) of tables[n_slots]
  * [max_pages] and lens[n_slots] (device arrays).  Token j of a slot lies in
  * page tables[slot][j / page_tokens]; tokens 0 .. lens[slot]-1 are attended to
- * (none: out 0, lse -inf).  The first `shared` tokens are the caller's promise
+ * (none: out 0, lse -inf); what other tokens of the pages hold does not matter.
+ * The first `shared` tokens are the caller's promise
  * to be the same for all sequences: they are read once for the batch, through
  * the pages of batch row 0's slot (whose row must hold them; with lens shorter
  * than `shared` a sequence sees only its first lens tokens).  Page numbers
  * outside the pool are read as page 0.  workspace: 256-byte aligned,
  * ane_attn_decode_workspace_size bytes, any contents, not shared by calls that
- * may overlap.  batch <= 1024; dim, heads, kv_heads as for ane_attn_prompt_dev. */
+ * may overlap.  batch <= 1024; scale, dim, heads, kv_heads as for
+ * ane_attn_prompt_dev. */
 size_t ane_attn_decode_workspace_size(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim);
 int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, float scale,
                         const ane_rows* q, const ane_pages* pages, const int32_t* tables, uint32_t n_slots,

@@ -107,6 +107,16 @@ def test_no_gpu_means_loud_failure():
     assert all(rc == NO_DEVICE for rc in calls(cache()))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.5, float("nan"), float("inf")])
+def test_scale_refusals(scale):
+    r, pages = rows(), ane.Pages(A, A, 16, 16, 2048, 128, 64)
+    assert L.ane_attn_prompt_dev(1, 1, 4, 2, 64, 10, 10, scale, P(r), P(r), P(r), A, None, 1, P(r), None, None, 0,
+                                 None) == INVALID
+    n = L.ane_attn_decode_workspace_size(2, 4, 2, 64)
+    assert L.ane_attn_decode_dev(1, 2, 4, 2, 64, scale, P(r), P(pages), A, 4, 8, A, None, 0, 1, P(r), None, A, n,
+                                 None) == INVALID
+
+
 def test_prompt_workspace():
     f = L.ane_attn_prompt_workspace_size
     assert f(1, 32, 32, 128, 17, 17) == 0  # nothing to split

@@ -347,3 +347,37 @@ def test_decode_long_prefix_many_rows(ane, lens, shared, heads, kv_heads, dim, p
     decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype)
     decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype, out_dtype=F32, want_lse=False, seed=2,
                 layout="heads")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dtype,dim", [(4, 4, F16, 128), (8, 2, BF16, 64)])
+@pytest.mark.parametrize("shared", [0, 37])
+def test_decode_neighbours_may_hold_anything(ane, heads, kv_heads, dtype, dim, shared):
+    """NaN, infinities and the type's lowest value in some sequences' own tokens
+    leave the others' bits alone, and show in their own results."""
+    lens = [shared + n for n in (70, 3, 129, 64, 1, 200, 17)]
+    q, k, v, tables, lens_t, slots, out = decode_case(ane, lens, shared, heads, kv_heads, dim, 16, dtype, seed=4)
+    clean = ane.attn_decode(q, k, v, tables, lens_t, slots=slots, shared=shared)
+    assert torch.equal(clean, out)
+    bad_rows = (1, 3, 5)
+    for bad in (float("nan"), float("inf"), -65504.0):
+        k2, v2, q2 = k.clone(), v.clone(), q.clone()
+        for b in bad_rows:
+            s = int(slots[b])
+            first = -(-shared // 16)  # pages of its own alone
+            pages = tables[s, first:-(-lens[b] // 16)].long()
+            if len(pages) == 0:
+                pages = tables[s, shared // 16:shared // 16 + 1].long()
+            v2[pages, :, :, 3] = bad
+            if bad == bad:  # NaN scores would make the whole row NaN: only V here
+                continue
+            k2[pages, 5:, :, 2] = bad
+            q2[b, :, 1] = bad
+        got = ane.attn_decode(q2, k2, v2, tables, lens_t, slots=slots, shared=shared)
+        for b in range(len(lens)):
+            if b not in bad_rows:
+                assert torch.equal(got[b], clean[b]), (bad, b)
+        if bad == float("inf"):
+            for b in bad_rows:
+                others = [c for c in range(dim) if c != 3]
+                assert not torch.isfinite(got[b, :, 3]).any()
+                assert torch.equal(got[b][:, others], clean[b][:, others])
