@@ -85,13 +85,13 @@ class KVCache:
         cache's type; cu None: one row per slot) become the last tokens of
         slots[i] on `layer`; rows of requests that were not granted are dropped."""
         n = slots.numel()
-        rows = ane._U64x6(*ane._rows("k", k, self.kv_heads, self.dim), *ane._rows("v", v, self.kv_heads, self.dim))
+        rk, rv = ane._rows("k", k, self.kv_heads, self.dim), ane._rows("v", v, self.kv_heads, self.dim)
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape and dtype")
         ane.check(ane.lib.ane_kv_write_dev(self._ref, layer, n, ane._i32_vector("slots", slots),
                                            None if cu is None else ane._i32_vector("cu", cu, n + 1),
                                            None if granted is None else ane._i32_vector("granted", granted, n),
-                                           k.shape[0], ane._dtype(k), ctypes.byref(rows), ctypes.byref(rows, 24),
+                                           k.shape[0], ane._dtype(k), rk, rv,
                                            ane._stream_of(stream, self.k)))
 
     def fork(self, parents, children, granted=None, stream=None):
