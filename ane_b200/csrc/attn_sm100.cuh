@@ -117,50 +117,59 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, uint8_t* dst, float f
                                            uint32_t dim, uint32_t out_dtype) {
     const int lane = threadIdx.x & 31;
     const uint32_t row_bytes = dim * (out_dtype == ANE_DTYPE_F32 ? 4 : 2), at0 = (lane & 7) * 16;
-    const bool zero = !any || factor == 0.0f;  // whatever the accumulator holds
-    const unsigned long long d = reinterpret_cast<unsigned long long>(dst);
+    const uint32_t keep = any && factor != 0.0f ? 0xffffffffu : 0u;  // 0 whatever the accumulator holds
+    const float2 f2 = make_float2(factor, factor);
     uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
+    unsigned long long to_row[8];  // of the rows that this lane stores
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        to_row[i] = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), i * 4 + (lane >> 3));
     auto flush = [&](uint32_t at) {  // the staged 128 bytes go to byte `at` of the rows
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int r = i * 4 + (lane >> 3);
-            const unsigned long long dr = __shfl_sync(0xffffffffu, d, r);
             const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            store16_if(dr && at + at0 < row_bytes, reinterpret_cast<uint8_t*>(dr) + at + at0, v);
+            store16_if(to_row[i] && at + at0 < row_bytes, reinterpret_cast<uint8_t*>(to_row[i]) + at + at0, v);
         }
         __syncwarp();
     };
-#pragma unroll 1
-    for (int c = 0; c < DP; c += 64) {
-        // one wait for 64 columns: each costs some 350 cycles next to running MMAs
-        // (read even if there is nothing: a branch here made the compiler spill)
-        uint32_t o[2][32];
-        ptx::tmem_ld_32x32b_x32(to + c, o[0]);
-        ptx::tmem_ld_32x32b_x32(to + c + 32, o[1]);
-        ptx::tmem_ld_wait();
-        ptx::pin32(o[0]);
-        ptx::pin32(o[1]);
+    // one wait for all columns: each costs some 350 cycles next to running MMAs
+    // (read even if there is nothing: a branch here made the compiler spill)
+    uint32_t o[DP / 32][32];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+    for (int c = 0; c < DP / 32; c++) ptx::tmem_ld_32x32b_x32(to + c * 32, o[c]);
+    ptx::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; i++) o[h][i] = zero ? 0u : __float_as_uint(__uint_as_float(o[h][i]) * factor);
-        if (out_dtype == ANE_DTYPE_F32) {
+    for (int c = 0; c < DP / 32; c++) ptx::pin32(o[c]);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+    for (int c = 0; c < DP / 32; c++)
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    mine[i ^ (lane & 7)] = make_uint4(o[h][4 * i], o[h][4 * i + 1], o[h][4 * i + 2], o[h][4 * i + 3]);
-                flush((c + h * 32) * 4);
-            }
-        } else {
+        for (int i = 0; i < 32; i += 2) {
+            const float2 y = ptx::fmul2(make_float2(__uint_as_float(o[c][i]), __uint_as_float(o[c][i + 1])), f2);
+            o[c][i] = __float_as_uint(y.x);
+            o[c][i + 1] = __float_as_uint(y.y);
+        }
+    if (out_dtype == ANE_DTYPE_F32) {
+#pragma unroll
+        for (int c = 0; c < DP / 32; c++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const uint32_t* x = &o[i >> 2][8 * (i & 3)];
-                mine[i ^ (lane & 7)] = make_uint4(pack_out<T>(x[0], x[1]), pack_out<T>(x[2], x[3]),
-                                                  pack_out<T>(x[4], x[5]), pack_out<T>(x[6], x[7]));
+                const uint32_t* x = &o[c][4 * i];
+                mine[i ^ (lane & 7)] = make_uint4(x[0] & keep, x[1] & keep, x[2] & keep, x[3] & keep);
             }
-            flush(c * 2);
+            flush(c * 128);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < DP / 32; c += 2) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t* x = &o[c + (i >> 2)][8 * (i & 3)];
+                mine[i ^ (lane & 7)] = make_uint4(pack_out<T>(x[0], x[1]) & keep, pack_out<T>(x[2], x[3]) & keep,
+                                                  pack_out<T>(x[4], x[5]) & keep, pack_out<T>(x[6], x[7]) & keep);
+            }
+            flush(c * 64);
         }
     }
 }
@@ -521,15 +530,15 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
                 l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
             }
             if (!ok) break;
+            uint8_t* dst = nullptr;
+            float factor = 0.0f;
+            if (real && token < it.tokens) job.result(it, row, token, m, l, kShift, dst, factor);
             if (begin < end) {
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.o_full[t], oc & 1, err));
                 if (!ok) break;
                 oc++;
                 ptx::tc_fence_after();
             }
-            uint8_t* dst = nullptr;
-            float factor = 0.0f;
-            if (real && token < it.tokens) job.result(it, row, token, m, l, kShift, dst, factor);
             store_rows<T, DP>(sm.out[warp], dst, factor, begin < end, to, job.dim(), job.out_dtype(it));
             ptx::tc_fence_before();
             __syncwarp();
