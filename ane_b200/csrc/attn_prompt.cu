@@ -30,6 +30,8 @@ struct Params {
     int* err;
     float *po, *pm;        // spans: parts, two per block (one that continues an item, one that begins it)
     struct Cut* cuts;      // spans: per block the item that it begins and does not end
+    uint32_t per_magic, per_shift;  // x / w, w = 2 * tile_tokens, is (x * magic >> 32) >> shift for x < 2^31:
+                                    // magic = ceil(2^(32 + shift) / w), 2^shift < w <= 2^(shift + 1)
 };
 
 struct Seq {
@@ -47,15 +49,17 @@ __device__ __forceinline__ Seq sequence(const Params& p, uint32_t s) {
     if (r.q0 < 0 || r.k0 < 0 || r.lq < 0) r.lq = 0;
     return r;
 }
+__device__ __forceinline__ int items_before(const Params& p, int token) {  // token >= 0
+    return (int)(__umulhi((uint32_t)token, p.per_magic) >> p.per_shift);
+}
 // Items of a sequence (per head) that need at least L key tiles.  Item i ends
 // with query token min((i + 1) * w, lq), whose last key is lk - lq + that.
-__device__ __forceinline__ int items_from_level(const Seq& s, int L, int w) {
-    const int n = (s.lq + w - 1) / w;
-    if (n == 0 || L <= 0) return n;
-    const int before = kBigKeys * (L - 1);
+__device__ __forceinline__ int items_from_level(const Params& p, const Seq& s, int L) {
+    if (s.lq == 0) return 0;
+    const int last = items_before(p, s.lq - 1), before = kBigKeys * (L - 1);
+    if (L <= 0) return last + 1;
     if (s.lk <= before) return 0;
-    const int x = before - (s.lk - s.lq);
-    return n - (x < 0 ? 0 : min(x / w, n - 1));
+    return last + 1 - min(items_before(p, max(before - (s.lk - s.lq), 0)), last);
 }
 
 // Room of a sequence's first k items (per head) on the line, in key tokens: what
@@ -86,6 +90,7 @@ struct Cut {
 struct PromptJob {
     const Params& p;
     Seq mine;  // of a searching warp: sequence `lane`, the first 32 of them kept
+    int level, above;        // whole items: `above` of them need at least `level` key tiles, all dealt out
     int64_t pos, end, span;  // spans: what is left of this block's, and their length
 
     __device__ Seq get(uint32_t s) const { return s < 32 ? mine : sequence(p, s); }
@@ -109,26 +114,43 @@ struct PromptJob {
         q.lk = __shfl_sync(0xffffffffu, q.lk, lane);
         return q;
     }
-    // Item number `o` in order of falling key tiles.  A whole warp.
-    __device__ BigItem find(int o) const {
+    // Item number `o` in order of falling key tiles, `o` not below the last
+    // call's: the search goes on from there (from scratch it took 3 to 6 us next to
+    // busy warps, longer than a short item).  A whole warp.
+    __device__ BigItem find(int o) {
         const int lane = threadIdx.x & 31, w = 2 * (int)p.tile_tokens;
         auto count = [&](int L) {
             int c = 0;
-            for (uint32_t s = lane; s < p.n_seq; s += 32) c += items_from_level(get(s), L, w);
+            for (uint32_t s = lane; s < p.n_seq; s += 32) c += items_from_level(p, get(s), L);
             return (int)__reduce_add_sync(0xffffffffu, c);
         };
         BigItem it{};
         it.head = -1;
-        if (count(0) <= o) return it;
-        int lo = 0, hi = (int)(p.total_k / kBigKeys) + 2;  // count(lo) > o >= count(hi)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (count(mid) > o) lo = mid; else hi = mid;
+        // the level that counts more than `o` items, below one that does not
+        int hi = level, below = above, lo;
+        for (int step = 1;; step *= 2) {
+            if (hi <= 0) return it;
+            lo = max(hi - step, 0);
+            const int c = count(lo);
+            if (c > o) break;
+            hi = lo;
+            below = c;
         }
-        int r = o - count(hi);
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1, c = count(mid);
+            if (c > o) {
+                lo = mid;
+            } else {
+                hi = mid;
+                below = c;
+            }
+        }
+        level = hi;
+        above = below;
+        int r = o - below;
         for (uint32_t s0 = 0; s0 < p.n_seq; s0 += 32) {
             const Seq q = get(s0 + lane);
-            const int a = items_from_level(q, lo, w), b = items_from_level(q, lo + 1, w);
+            const int a = items_from_level(p, q, lo), b = items_from_level(p, q, hi);
             int sum = a - b;
             for (int d = 1; d < 32; d <<= 1) {
                 const int t = __shfl_up_sync(0xffffffffu, sum, d);
@@ -138,8 +160,9 @@ struct PromptJob {
             if (hit) {
                 const int l = __ffs((int)hit) - 1;
                 const Seq one = broadcast(q, l);
-                const int n = (one.lq + w - 1) / w;
-                fill(it, one, (n - __shfl_sync(0xffffffffu, a, l) + r - __shfl_sync(0xffffffffu, sum - (a - b), l)) * w);
+                const int last = items_before(p, max(one.lq - 1, 0));
+                const int x = last + 1 - __shfl_sync(0xffffffffu, a, l) + r - __shfl_sync(0xffffffffu, sum - (a - b), l);
+                fill(it, one, min(max(x, 0), last) * w);  // (sums pass 2^31 only for ranges that overlap)
                 return it;
             }
             r -= __shfl_sync(0xffffffffu, sum, 31);
@@ -202,14 +225,18 @@ struct PromptJob {
                 pos = min(all, span * blockIdx.x);
                 end = min(all, span * (blockIdx.x + 1));
                 if ((threadIdx.x & 31) == 0) p.cuts[blockIdx.x].span = 0;
+            } else {
+                level = above = 0;
+                for (uint32_t s = threadIdx.x & 31; s < p.n_seq; s += 32) level = max(level, get(s).lk);
+                level = __reduce_max_sync(0xffffffffu, level) / kBigKeys + 2;
             }
         }
         BigItem it{};
         it.head = -1;
         if (!p.spans) {
             const uint64_t w = (uint64_t)i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-            if (w < 0x7fffffffu) it = find((int)(w / p.kv_heads));
-            if (it.head >= 0) it.head = (int)(w % p.kv_heads);
+            if (w < 0x7fffffffu) it = find((int)((uint32_t)w / p.kv_heads));
+            if (it.head >= 0) it.head = (int)((uint32_t)w % p.kv_heads);
             it.slot = -1;
             return it;
         }
@@ -264,7 +291,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kBigThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const Params p) {
-    PromptJob job{p, {0, 0, 0, 0}, 0, 0, 0};
+    PromptJob job{p};
     big_attention<T, DP>(&map_q, &map_k, &map_v, p.group, p.scale2, p.err, job);
 }
 
@@ -325,7 +352,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
             o[i].w = o[i].w * ca + v[i].w * cb;
         }
     }
-    const PromptJob job{p, {0, 0, 0, 0}, 0, 0, 0};
+    const PromptJob job{p};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int token = t * (int)p.tile_tokens + (row + i) / (int)p.group;
@@ -420,6 +447,9 @@ extern "C" int ane_attn_prompt_dev(uint32_t dtype, uint32_t n_seq, uint32_t head
     Params p{n_seq, heads, kv_heads, group, dim, total_q, total_k, out_dtype, 128 / group,
              spans_for(n_seq, group, kv_heads, total_q, total_k), scale * attn::kLog2e, *out, cu_q,
              cu_k ? cu_k : cu_q, lse, device_timeout_flag()};
+    const uint32_t w = 2 * p.tile_tokens;
+    while ((2u << p.per_shift) < w) p.per_shift++;
+    p.per_magic = (uint32_t)(((1ull << (32 + p.per_shift)) + w - 1) / w);
     if (p.spans) {
         p.po = static_cast<float*>(workspace);
         p.pm = p.po + (size_t)p.spans * 4 * kBigRows * dim;
