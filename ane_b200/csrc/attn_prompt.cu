@@ -372,8 +372,9 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 // many items total_q tokens in n_seq pieces can make and how long a key line can
 // be.  From three items per SM dealing whole items out loses less than the parts
 // and their join cost (8 ragged prompts of up to 1531 tokens, 3 to 4 items per SM:
-// 57 us whole, 81 us as spans; 2 blocks of up to 1024 tokens behind 7681, 1.3 items
-// per SM: 209 us whole, 188 us as spans).
+// 46 us whole, 75 us as spans; 2 blocks of up to 1024 tokens behind 7681, 1.3 items
+// per SM and all of them long: 198 us whole, 169 us as spans; 2 prompts of 1000-4000
+// tokens, 8 heads, 1.6 items per SM of any length: 78 and 86).
 constexpr uint32_t kSpanKeys = 1024;
 uint32_t spans_for(uint32_t n_seq, uint32_t group, uint32_t kv_heads, uint32_t total_q, uint32_t total_k) {
     const uint64_t items = (uint64_t)(total_q / (2 * (kBigRows / group)) + n_seq) * kv_heads;
