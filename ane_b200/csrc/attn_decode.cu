@@ -45,13 +45,13 @@ struct Params {
     uint32_t groups, subs;   // units per key/value head: groups of sequences x parts of 16 heads
     uint32_t rows;           // rows of a unit's partial result
     uint32_t whole;          // 1: a block per unit, results written
+    uint32_t blocks;         // of decode_kernel
     uint32_t big_splits;     // spans of prefix_kernel (0: not used)
     uint32_t n_slots, max_pages, pages, page_shift, box_keys;
     float scale2;
     ane_rows q, out;
     const int32_t *tables, *lens, *slots;
     float* lse;
-    int32_t* cum;       // [batch + 1] own tiles of the sequences before b; then steps per block
     float *po, *pm;     // prefix_kernel's partials: rows x dim; rows x {m, l}
     float *so, *sm;     // decode_kernel's
     int* err;
@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     // which may hold what they were before); it waits for prefix_kernel itself
     // only at the end.
     if (p.big_splits == 0) {
+        ptx::griddep_wait();  // in this order: join_kernel reads the lengths without waiting
         ptx::griddep_launch_dependents();
-        ptx::griddep_wait();
     }
     for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) {
         const int2 q = seq_of(p, b);
@@ -337,10 +337,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int per_g = (int)(p.kv_heads * p.subs);  // units of a group
     const int total = group_start(p, sm.cum, p.groups) * per_g;
     const int per = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
-    if (blockIdx.x == 0 && !p.whole) {
-        for (uint32_t b = threadIdx.x; b <= p.batch; b += kThreads) p.cum[b] = sm.cum[b];
-        if (threadIdx.x == 0) p.cum[p.batch + 1] = per;
-    }
 
     if (warp >= 4) {
         // -------------------------------------------------------- producers
@@ -726,8 +722,8 @@ __global__ void __launch_bounds__(kBigThreads, 1)
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     __shared__ float sm_m[4], sm_l[4], sm_o[4][128];
+    __shared__ int sm_tiles[4][3];
     ptx::griddep_launch_dependents();
-    ptx::griddep_wait();
     const uint32_t b = blockIdx.x, head = blockIdx.y, h = head / p.group, g = head % p.group;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // spans [pc, pe) of prefix_kernel and [oc, oe) of decode_kernel's blocks hold
@@ -737,9 +733,28 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const size_t prow = (size_t)h * all_rows + b * p.group + g, pstep = all_rows * p.kv_heads;
     const uint32_t grp = b / p.per_unit, sub = p.group > 16 ? g / 16 : 0;
     const uint32_t row = p.group > 16 ? g % 16 : b % p.per_unit * p.group + g;
-    const int per = __ldcg(p.cum + p.batch + 1), per_g = (int)(p.kv_heads * p.subs), id = (int)(h * p.subs + sub);
-    const int c0 = __ldcg(p.cum + min(grp * p.per_unit, p.batch)), c1 = __ldcg(p.cum + min((grp + 1) * p.per_unit, p.batch));
-    const int n = c1 - c0 + (int)p.prefix_tiles;  // tiles of the row's unit
+    // Where decode_kernel's blocks cut the line, from the lengths, while they end:
+    // own tiles of the sequences before the row's unit, of the unit and of all.
+    int tiles[3] = {0, 0, 0};
+    for (uint32_t x = threadIdx.x; x < p.batch; x += kJoinThreads) {
+        const int own = own_tiles(p, len_of(p, x)), u = (int)(x / p.per_unit) - (int)grp;
+        tiles[0] += u < 0 ? own : 0;
+        tiles[1] += u == 0 ? own : 0;
+        tiles[2] += own;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        tiles[i] = __reduce_add_sync(0xffffffffu, tiles[i]);
+        if (lane == 0) sm_tiles[warp][i] = tiles[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; i++) tiles[i] = sm_tiles[0][i] + sm_tiles[1][i] + sm_tiles[2][i] + sm_tiles[3][i];
+    ptx::griddep_wait();
+    const int per_g = (int)(p.kv_heads * p.subs), id = (int)(h * p.subs + sub), c0 = tiles[0];
+    const int total = ((int)(p.groups * (kUnitCost + p.prefix_tiles)) + tiles[2]) * per_g;
+    const int per = (int)(((unsigned)total + p.blocks - 1) / p.blocks);
+    const int n = tiles[1] + (int)p.prefix_tiles;  // tiles of the row's unit
     int oc = 0, oe = 0;
     if (n) {
         const int first = ((int)(grp * (kUnitCost + p.prefix_tiles)) + c0) * per_g + id * (n + kUnitCost) + kUnitCost;
@@ -807,7 +822,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
 // ------------------------------------------------------------------ launch
 struct Layout {
     uint32_t per_unit, groups, subs, rows, pairs, big_splits;
-    size_t cum, pm, po, sm, so, bytes;
+    size_t pm, po, sm, so, bytes;
 };
 Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
     Layout l;
@@ -827,7 +842,6 @@ Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
         at += round_up(bytes, 256);
         return here;
     };
-    l.cum = take((batch + 2) * 4);
     l.pm = take(prefix_rows * 8);
     l.sm = take(own_rows * 8);
     l.po = take(prefix_rows * dim * 4);
@@ -849,9 +863,7 @@ int launch(const CUtensorMap (&map)[3], const Params& p, uint32_t pairs, cudaStr
             return rc;
     }
     if ((rc = set_max_dynamic_smem(decode_kernel<T, DP>, (int)decode_smem_bytes<DP>(), done))) return rc;
-    const uint32_t spans = (uint32_t)num_sms() * 2 < kMaxBlocks ? (uint32_t)num_sms() * 2 : kMaxBlocks;
-    const uint32_t blocks = p.whole ? p.kv_heads * p.groups * p.subs : spans;
-    if ((rc = launch_pdl(decode_kernel<T, DP>, dim3(blocks), dim3(kThreads), decode_smem_bytes<DP>(), s, map[1], map[2], p)) ||
+    if ((rc = launch_pdl(decode_kernel<T, DP>, dim3(p.blocks), dim3(kThreads), decode_smem_bytes<DP>(), s, map[1], map[2], p)) ||
         p.whole)
         return rc;
     return launch_pdl(join_kernel<T>, dim3(p.batch, p.heads), dim3(kJoinThreads), 0, s, p);
@@ -923,7 +935,6 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.scale2 = scale * attn::kLog2e;
     p.q = *q, p.out = *out;
     p.tables = tables, p.lens = lens, p.slots = slots, p.lse = lse;
-    p.cum = reinterpret_cast<int32_t*>(ws + l.cum);
     p.pm = reinterpret_cast<float*>(ws + l.pm), p.po = reinterpret_cast<float*>(ws + l.po);
     p.sm = reinterpret_cast<float*>(ws + l.sm), p.so = reinterpret_cast<float*>(ws + l.so);
     p.err = device_timeout_flag();
@@ -931,6 +942,8 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.box_keys = pt < (uint32_t)kTile ? pt : (uint32_t)kTile;
     const uint64_t own = ceil_div(most - (shared & ~(p.box_keys - 1)), kTile);  // of a sequence, at most
     p.whole = !big && p.prefix_tiles + (batch < l.per_unit ? batch : l.per_unit) * own <= kWholeTiles;
+    const uint32_t spans = (uint32_t)num_sms() * 2;
+    p.blocks = p.whole ? kv_heads * l.groups * l.subs : spans < kMaxBlocks ? spans : kMaxBlocks;
     const auto type = dtype == ANE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     CUtensorMap map[3];
     if (big && (rc = encode_tensor_map_3d(&map[0], type, q->data, {dim, heads, batch},
