@@ -34,8 +34,9 @@ constexpr uint32_t kKept = 256;        // sequences whose slot and length stay i
 constexpr int kPagesAhead = 4;         // tiles whose page numbers are read ahead
 constexpr int kUnits = 4;              // units announced ahead
 constexpr int kUnitCost = 2;           // a unit's start and end cost about what two tiles do
-constexpr uint32_t kWholeTiles = 10;   // units of at most so many tiles are not cut: 10 tiles take about
-                                       // what a second launch and the joining do
+constexpr uint32_t kWholeTiles = 7;    // units of at most so many tiles are not cut (2 sequences x 32 heads in a
+                                       // graph, tiles a unit: whole and cut; 7: 12.3 and 12.3 us, 9: 14.3 and
+                                       // 12.3); a cut call costs the host a second launch
 
 struct Params {
     uint32_t batch, heads, kv_heads, group, dim, out_dtype;
@@ -917,9 +918,9 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.shared = shared;
     // decode_kernel goes over the prefix once per unit of 16 rows.  The second time costs
     // little (L2), every further one a tile's time: prefix_kernel from where that
-    // makes eight tiles a block.  128 rows x 8 heads, 4096 shared: 31 us without it,
-    // 25 with it; 1024 shared: 23 and 23; 64 rows x 32 heads, 1024 shared: 41 and 44;
-    // 32 rows x 32 heads, 16384 shared: 74 and 86.
+    // makes eight tiles a block.  128 rows x 8 heads, 4096 shared: 29 us without it,
+    // 25 with it; 2048 shared: 23 and 25; 64 rows x 32 heads, 1024 shared: 33 and 36;
+    // 32 rows x 32 heads, 16384 shared: 70 and 86.
     const uint32_t units = l.groups * l.subs;
     const uint64_t again = units > 2 ? (uint64_t)(units - 2) * kv_heads * ceil_div(shared, kTile) : 0;
     const bool big = again >= 8 * 2 * (uint64_t)kBigBlocks;
