@@ -342,7 +342,7 @@ def test_decode_full_batch(ane):
     ([4100 + b for b in range(70)] + [0, 100, 4096], 4096, 8, 8, 64, 16, F16),
     ([1500 + 50 * (b % 9) for b in range(130)], 1411, 20, 4, 80, 8, F16),  # 5 heads a group: 125 rows per tile
     ([2048] * 64, 2048, 32, 8, 128, 256, BF16),                           # nothing of their own
-    # an odd number of row tiles, the last of which takes two spans of the prefix at a time:
+    # an odd number of row tiles (the last is alone in its pair):
     ([870 + 9 * (b % 50) for b in range(95)] + [500], 870, 32, 8, 128, 32, F16),  # fewer key tiles than spans
     ([9001 + b for b in range(5)], 9001, 64, 1, 128, 64, BF16),
     ([700 + b % 70 for b in range(130)], 700, 128, 64, 64, 8, BF16),       # more items than SMs
