@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Pool p, uint32_t layer,
     ptx::griddep_wait();
     const int32_t t = (int32_t)blockIdx.x;
     uint32_t lo = cu ? 0 : blockIdx.x, hi = cu ? n - 1 : blockIdx.x;
-    if (cu && t >= cu[n]) return;
+    if (cu && (t < cu[0] || t >= cu[n])) return;  // rows of no request
     while (lo < hi) {
         const uint32_t mid = (lo + hi + 1) >> 1;
         if (cu[mid] <= t) lo = mid; else hi = mid - 1;

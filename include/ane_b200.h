@@ -530,8 +530,9 @@ int ane_kv_reserve_dev(const ane_kv_cache* cache, uint32_t n, const int32_t* slo
                        int32_t* granted, void* stream);
 /* Writes rows cu[i] .. cu[i+1]-1 of k and v (F32, rounded to nearest, or the
  * cache's type) to the last cu[i+1]-cu[i] tokens of slots[i] on one layer (cu
- * NULL: one row per request).  granted (NULL: all) as ane_kv_reserve_dev left
- * it: rows of refused requests are dropped.  tokens: rows that k and v hold. */
+ * NULL: one row per request; rows before cu[0] and from cu[n] on are nobody's).
+ * granted (NULL: all) as ane_kv_reserve_dev left it: rows of refused requests
+ * are dropped.  tokens: rows that k and v hold. */
 int ane_kv_write_dev(const ane_kv_cache* cache, uint32_t layer, uint32_t n, const int32_t* slots, const int32_t* cu,
                      const int32_t* granted, uint32_t tokens, uint32_t src_dtype, const ane_rows* k,
                      const ane_rows* v, void* stream);

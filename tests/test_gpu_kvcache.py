@@ -286,3 +286,26 @@ def test_graph_and_side_stream(ane):
     m.free([1, 2])
     m.same(c)
     assert granted.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("src", [torch.float32, torch.float16])
+def test_write_leaves_rows_outside_cu_alone(ane, src):
+    """Rows before cu[0] and from cu[n] on belong to no request: a slot's older
+    tokens, and the pages that a fork reads with it, stay as they are."""
+    c = new_cache(layers=2, pages=20, page=16, heads=2, dim=64, slots=4, max_pages=6)
+    m = Model(c)
+    assert c.reserve(i32([0]), i32([37])).tolist() == m.reserve([0], [37])
+    assert c.fork(i32([0]), i32([1])).tolist() == m.fork([0], [1])
+    slots, cu = [0, 2], [26, 31, 34]  # as many rows before them as reach the whole pages that slot 1 reads too
+    granted = c.reserve(i32(slots), i32([5, 3]))
+    assert granted.tolist() == m.reserve(slots, [5, 3])
+    rows = torch.randn(40, 4, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(src)
+    k, v = rows[:, :2], rows[:, 2:]
+    c.write(1, i32(slots), k, v, cu=i32(cu), granted=granted)
+    for i, s in enumerate(slots):
+        n = cu[i + 1] - cu[i]
+        for j in range(n):
+            t = m.lens[s] - n + j
+            m.k[1, m.tables[s][t // 16], t % 16] = k[cu[i] + j].half()
+            m.v[1, m.tables[s][t // 16], t % 16] = v[cu[i] + j].half()
+    m.same(c)
