@@ -4,7 +4,8 @@
 // decode_kernel works on units of at most 16 query rows (as many sequences as
 // fit, with the heads that share a key/value head) on mma.sync: a unit's keys are
 // the shared prefix, which all of its rows see, and then each of its sequences'
-// own tokens, which only that sequence's rows see.  It is bound by the bytes of K
+// own tokens, which only that sequence's rows see.  (A sequence that ends inside
+// the prefix has all its tokens as its own.)  It is bound by the bytes of K
 // and V, so all units' 64-token tiles are laid end to end and cut into equal
 // spans, one per block: ragged lengths and a single long sequence load the chip
 // alike.  Two producer warps stream a span's tiles through a ring by TMA, across
@@ -68,10 +69,16 @@ __device__ __forceinline__ int2 seq_of(const Params& p, uint32_t b) {
     return make_int2(s, s < 0 ? 0 : min(max(__ldcg(p.lens + s), 0), (int)(p.max_pages << p.page_shift)));
 }
 __device__ __forceinline__ int len_of(const Params& p, uint32_t b) { return seq_of(p, b).y; }
+// Keys of the prefix that a sequence's rows see as such: all or none.  With some
+// of them, V of the others would meet a weight of 0 in the products, which does not
+// silence an infinity or NaN there.
+__device__ __forceinline__ int prefix_seen(const Params& p, int len) { return len < (int)p.shared ? 0 : (int)p.shared; }
 // Own tiles start where the box of tokens does that holds the first own one.
-__device__ __forceinline__ int own_base(const Params& p) { return (int)(p.shared & ~(p.box_keys - 1)); }
+__device__ __forceinline__ int own_base(const Params& p, int len) {
+    return prefix_seen(p, len) & ~((int)p.box_keys - 1);
+}
 __device__ __forceinline__ int own_tiles(const Params& p, int len) {
-    return len > (int)p.shared ? (len - own_base(p) + kTile - 1) / kTile : 0;
+    return len == (int)p.shared ? 0 : (len - own_base(p, len) + kTile - 1) / kTile;
 }
 // Place on the line where the units of group g begin, counted per head and part.
 // cum: own tiles of the sequences before b.
@@ -408,8 +415,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         auto own = [&](int b) { return sm.cum[b + 1] - sm.cum[b]; };
         auto to_sequence = [&](Cursor& c, const Unit& u, int b, int skip) {
             const int2 q = seq((uint32_t)b);
-            c.t = Tile{b - u.grp * (int)p.per_unit, own_base(p) + skip * kTile, (int)p.shared, q.y};
-            c.table = p.tables + (size_t)max(q.x, 0) * p.max_pages;
+            const int seen = prefix_seen(p, q.y);
+            c.t = Tile{b - u.grp * (int)p.per_unit, own_base(p, q.y) + skip * kTile, seen, q.y};
+            c.table = p.tables + (size_t)max(q.y < (int)p.shared ? seq(0).x : q.x, 0) * p.max_pages;
             c.left = own(b) - skip;
         };
         auto seek = [&](const Unit& u) {  // u has tiles
@@ -528,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ptx::smem_u32(&sm.q_full[to])) : "memory");
             if (warp == 0) {
                 if (lane < 16)
-                    sm.vis[to][lane] = row_of(p, dst.grp, dst.sub, sm.place[lane], b, g) ? min(seq(b).y, (int)p.shared) : 0;
+                    sm.vis[to][lane] = row_of(p, dst.grp, dst.sub, sm.place[lane], b, g) ? prefix_seen(p, seq(b).y) : 0;
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&sm.q_full[to]);
             }
@@ -576,6 +584,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 __syncwarp();
                 if (t + 1 < u.t1 && lane == 0) ptx::mbar_arrive(&sm.empty[st]);
+                // rows that have seen nothing so far start from 0, whatever the prefix's V made of their weights of 0
+                if (t + 1 == (int)p.prefix_tiles || t + 1 == u.t1) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int i = 0; i < DP / 8; i++)
+                            if (r.m[h] == kNegInf) r.o[i][2 * h] = r.o[i][2 * h + 1] = 0.0f;
+                }
                 if (t == u.t0) fetch(un);
                 if (!ok) break;
             }
@@ -696,7 +712,7 @@ struct PrefixJob {
         return page_of(p, p.tables + (size_t)max(s, 0) * p.max_pages, min(key, (int)p.shared - 1) & ~((int)p.box_keys - 1));
     }
     __device__ int visible(const BigItem& it, int token) const {
-        return min(len_of(p, (uint32_t)(it.q_token + token)), (int)p.shared);
+        return prefix_seen(p, len_of(p, (uint32_t)(it.q_token + token)));
     }
     __device__ void result(const BigItem& it, int row, int token, float m, float l, float shift, uint8_t*& dst,
                            float& factor) const {

@@ -489,7 +489,8 @@ typedef struct ane_pages {
  * The first `shared` tokens are the caller's promise
  * to be the same for all sequences: they are read once for the batch, through
  * the pages of batch row 0's slot (whose row must hold them; with lens shorter
- * than `shared` a sequence sees only its first lens tokens).  Page numbers
+ * than `shared` a sequence sees only its first lens tokens, which are then read
+ * for it alone).  Page numbers
  * outside the pool are read as page 0.  workspace: 256-byte aligned,
  * ane_attn_decode_workspace_size bytes, any contents, not shared by calls that
  * may overlap.  batch <= 1024; scale, dim, heads, kv_heads as for

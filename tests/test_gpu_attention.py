@@ -386,3 +386,40 @@ def test_decode_neighbours_may_hold_anything(ane, heads, kv_heads, dtype, dim, s
                 others = [c for c in range(dim) if c != 3]
                 assert not torch.isfinite(got[b, :, 3]).any()
                 assert torch.equal(got[b][:, others], clean[b][:, others])
+
+
+SHORT = [
+    # lens, shared, heads, kv_heads, dim, page, dtype
+    ([130, 40, 0, 100, 137, 1, 64], 100, 4, 4, 128, 16, F16),     # all rows in one unit
+    ([700, 90, 640, 300, 65], 600, 8, 2, 64, 32, BF16),           # tiles that a row sees in part, and not at all
+    ([400, 33, 399], 333, 24, 1, 80, 8, F16),                     # units of one sequence
+    ([1000, 1], 900, 2, 2, 128, 64, BF16),
+    ([4100 + b % 9 for b in range(38)] + [0, 100, 4095, 1, 2048], 4096, 32, 8, 64, 16, F16),  # prefix_kernel
+    ([2700 + 13 * b for b in range(31)] + [2600, 2599, 77], 2600, 64, 8, 128, 64, BF16),
+]
+
+
+@pytest.mark.parametrize("lens,shared,heads,kv_heads,dim,page,dtype", SHORT)
+def test_decode_short_sequences_do_not_see_the_rest_of_the_prefix(ane, lens, shared, heads, kv_heads, dim, page, dtype):
+    """What the shared tokens past a sequence's own length hold leaves its bits
+    alone; sequences that see them show it in that column alone."""
+    q, k, v, tables, lens_t, slots, out = decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype, seed=6)
+    table = tables[int(slots[0])].tolist()
+    for cut in sorted({n for n in lens if 0 < n < shared}):
+        for bad in (float("nan"), float("inf"), -torch.finfo(dtype).max):
+            for hit_k in (False, True):
+                k2, v2 = k.clone(), v.clone()
+                for t in {cut, cut + 1, (cut + shared) // 2, shared - 1}:
+                    if t < cut or t >= shared:
+                        continue
+                    v2[table[t // page], t % page, :, 3] = bad
+                    if hit_k:
+                        k2[table[t // page], t % page, :, 2] = bad
+                got = ane.attn_decode(q, k2, v2, tables, lens_t, slots=slots, shared=shared)
+                for b, n in enumerate(lens):
+                    if n <= cut:
+                        assert torch.equal(got[b], out[b]), (cut, bad, hit_k, b)
+                    elif not hit_k and n >= shared:
+                        others = [c for c in range(dim) if c != 3]
+                        assert torch.equal(got[b][:, others], out[b][:, others]), (cut, bad, b)
+                        assert bad == bad and abs(bad) < 1e39 or not torch.isfinite(got[b, :, 3]).any()
