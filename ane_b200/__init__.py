@@ -656,7 +656,8 @@ def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, 
     heads, dim], one layer's pages k and v [pages, page_tokens, kv_heads, dim],
     tables int32 [n_slots, max_pages], lens int32 [n_slots], row b of the batch
     in slot slots[b] (default b).  The first `shared` tokens are the same for the
-    whole batch and are read once, through the pages of row 0's slot."""
+    whole batch and are read once, through the pages of the first row that holds
+    them all (a sequence may have fewer: it sees those)."""
     B, heads, dim = q.shape
     pages, page_tokens, kv_heads, kd = k.shape
     sp, st, sh, sd = strides = k.stride()

@@ -85,6 +85,21 @@ __device__ __forceinline__ int own_tiles(const Params& p, int len) {
 __device__ __forceinline__ int group_start(const Params& p, const int32_t* cum, uint32_t g) {
     return (int)(g * (kUnitCost + p.prefix_tiles)) + cum[min(g * p.per_unit, p.batch)];
 }
+// Slot through whose pages the prefix is read: the first sequence that reaches its
+// end, or the first of those that reach farthest (the others may be idle, and their
+// table rows stale).  A whole warp; seq(b): {slot, tokens}.
+template <class Seq>
+__device__ __forceinline__ int prefix_slot(const Params& p, Seq seq) {
+    uint32_t most = 0, at = 0;
+    int slot = 0;
+    for (uint32_t b = threadIdx.x & 31; b < p.batch; b += 32) {
+        const int2 q = seq(b);
+        const uint32_t n = min((uint32_t)q.y, p.shared);
+        if (n > most) most = n, at = b, slot = q.x;
+    }
+    const uint32_t first = __reduce_min_sync(0xffffffffu, most == __reduce_max_sync(0xffffffffu, most) ? at : ~0u);
+    return __shfl_sync(0xffffffffu, slot, (int)(first & 31));
+}
 // A unit's row: sequence (of the unit) and head (of its part of 16, or of the
 // group); the same for all units.
 struct RowPlace {
@@ -130,6 +145,7 @@ struct DecodeSmem {
     float2 ml[kStages][4][16];       // {m, l} of each warp's rows
     int cum[kMaxBatch + 1];          // own tiles of the sequences before b
     int2 seq[kKept];                 // {slot, len} of the first sequences
+    int prefix_slot;
     Unit unit[kUnits];
     Tile tile[kStages];
     RowPlace place[16];
@@ -340,6 +356,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             base += __shfl_sync(0xffffffffu, s, 31);
         }
         if (lane == 0) sm.cum[p.batch] = base;
+    } else if (warp == 1 && p.shared) {
+        const int slot = prefix_slot(p, seq);
+        if (lane == 0) sm.prefix_slot = slot;
     }
     __syncthreads();
     const int per_g = (int)(p.kv_heads * p.subs);  // units of a group
@@ -417,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int2 q = seq((uint32_t)b);
             const int seen = prefix_seen(p, q.y);
             c.t = Tile{b - u.grp * (int)p.per_unit, own_base(p, q.y) + skip * kTile, seen, q.y};
-            c.table = p.tables + (size_t)max(q.y < (int)p.shared ? seq(0).x : q.x, 0) * p.max_pages;
+            c.table = p.tables + (size_t)max(q.y < (int)p.shared ? sm.prefix_slot : q.x, 0) * p.max_pages;
             c.left = own(b) - skip;
         };
         auto seek = [&](const Unit& u) {  // u has tiles
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             int t = u.t0, b = u.grp * (int)p.per_unit;
             if (t < (int)p.prefix_tiles) {
                 c.t = Tile{-1, t * kTile, 0, (int)p.shared};
-                c.table = p.tables + (size_t)max(seq(0).x, 0) * p.max_pages;
+                c.table = p.tables + (size_t)sm.prefix_slot * p.max_pages;
                 c.left = (int)p.prefix_tiles - t;
                 return c;
             }
@@ -686,6 +705,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 struct PrefixJob {
     const Params& p;
     uint32_t pairs;  // items along the rows: two tiles of 128 / group sequences each
+    const int32_t* table;
+
+    __device__ void start() {
+        table = p.tables + (size_t)prefix_slot(p, [&](uint32_t b) { return seq_of(p, b); }) * p.max_pages;
+    }
 
     __device__ BigItem item(int i) const {
         const uint32_t tt = kBigRows / p.group, w = (uint32_t)i * gridDim.x + blockIdx.x;  // split, head, pair
@@ -708,8 +732,7 @@ struct PrefixJob {
     }
     __device__ int box_keys() const { return (int)p.box_keys; }
     __device__ int2 coord(const BigItem& it, int key) const {
-        const int s = slot_of(p, 0);
-        return page_of(p, p.tables + (size_t)max(s, 0) * p.max_pages, min(key, (int)p.shared - 1) & ~((int)p.box_keys - 1));
+        return page_of(p, table, min(key, (int)p.shared - 1) & ~((int)p.box_keys - 1));
     }
     __device__ int visible(const BigItem& it, int token) const {
         return prefix_seen(p, len_of(p, (uint32_t)(it.q_token + token)));
@@ -730,7 +753,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kBigThreads, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const Params p, uint32_t pairs) {
-    PrefixJob job{p, pairs};
+    PrefixJob job{p, pairs, nullptr};
     big_attention<T, DP>(&map_q, &map_k, &map_v, p.group, p.scale2, p.err, job);
 }
 

@@ -93,6 +93,7 @@ struct PromptJob {
     int level, above;        // whole items: `above` of them need at least `level` key tiles, all dealt out
     int64_t pos, end, span;  // spans: what is left of this block's, and their length
 
+    __device__ void start() const {}
     __device__ Seq get(uint32_t s) const { return s < 32 ? mine : sequence(p, s); }
     __device__ void fill(BigItem& it, const Seq& q, int first) const {
         const int tt = (int)p.tile_tokens;

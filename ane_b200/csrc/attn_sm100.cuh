@@ -175,6 +175,7 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, uint8_t* dst, float f
 }
 
 // The kernel's frame.  Job supplies:
+//   start()                     called by the loading warp before coord
 //   item(i)                     item i of this block (a whole warp; head -1: no more)
 //   box_keys()                  keys per TMA box (a multiple of 8 that divides 128)
 //   coord(item, key)            {token, page} coordinates of the box that starts at a key
@@ -245,6 +246,7 @@ __device__ __forceinline__ void big_attention(const CUtensorMap* map_q, const CU
         if (warp == 8) {
             // ---------------------------------------------------------- loads
             // one lane per box: 64 elements x box_keys keys
+            job.start();
             const int box_keys = job.box_keys(), boxes = kBigKeys / box_keys * kBoxes;
             const int key0 = lane / kBoxes * box_keys, x0 = lane % kBoxes * 64;
             const uint32_t dst0 = lane % kBoxes * kBoxBytes + key0 * 128;

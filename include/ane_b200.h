@@ -488,9 +488,9 @@ typedef struct ane_pages {
  * (none: out 0, lse -inf); what other tokens of the pages hold does not matter.
  * The first `shared` tokens are the caller's promise
  * to be the same for all sequences: they are read once for the batch, through
- * the pages of batch row 0's slot (whose row must hold them; with lens shorter
- * than `shared` a sequence sees only its first lens tokens, which are then read
- * for it alone).  Page numbers
+ * the pages of the first batch row that holds them all (lens >= shared; if none
+ * does, the first that holds most).  A sequence with fewer tokens than `shared`
+ * sees only those, read through the same pages for it alone.  Page numbers
  * outside the pool are read as page 0.  workspace: 256-byte aligned,
  * ane_attn_decode_workspace_size bytes, any contents, not shared by calls that
  * may overlap.  batch <= 1024; scale, dim, heads, kv_heads as for

@@ -423,3 +423,48 @@ def test_decode_short_sequences_do_not_see_the_rest_of_the_prefix(ane, lens, sha
                         others = [c for c in range(dim) if c != 3]
                         assert torch.equal(got[b][:, others], out[b][:, others]), (cut, bad, b)
                         assert bad == bad and abs(bad) < 1e39 or not torch.isfinite(got[b, :, 3]).any()
+
+
+def check_decode(ane, q, k, v, tables, lens, slots, shared, holder, **kw):
+    """attn_decode against the definition; the shared tokens are those of batch row `holder`."""
+    B, heads, dim = q.shape
+    page, kv_heads = k.shape[1:3]
+    group = heads // kv_heads
+    lse = torch.full((B, heads), 7.0, device="cuda")
+    out = ane.attn_decode(q, k, v, tables, lens, slots=slots, shared=shared, lse=lse, **kw)
+    for b, s in enumerate(slots.tolist()):
+        n = int(lens[s]) if 0 <= s < len(lens) else 0
+        t = torch.arange(n, device="cuda")
+        row = torch.where(t < shared, int(slots[holder]), s)
+        pages = tables[row, t // page].long()
+        ks, vs = k[pages, t % page], v[pages, t % page]
+        visible = torch.full((group,), n, device="cuda")
+        for h in range(kv_heads):
+            a, e = h * group, (h + 1) * group
+            check_rows(out[b, a:e], q.dtype, q[b, a:e], ks[:, h], vs[:, h], dim ** -0.5, visible, lse[b, a:e])
+    return out
+
+
+@pytest.mark.parametrize("lens,shared,heads,kv_heads,dim,page,dtype", [
+    ([180, 0, 40, 150, 131], 129, 4, 4, 128, 16, F16),
+    ([700, 90, 640, 0, 620], 600, 8, 2, 64, 32, BF16),
+    ([64, 20, 1, 0], 64, 4, 4, 128, 16, F16),
+    ([4100 + b % 9 for b in range(38)] + [0, 100, 4095, 1, 2048], 4096, 32, 8, 64, 16, F16),
+    ([2700 + 13 * b for b in range(31)] + [2600, 2599, 0], 2600, 64, 8, 128, 64, BF16),
+])
+def test_decode_prefix_of_a_row_that_holds_it(ane, lens, shared, heads, kv_heads, dim, page, dtype):
+    """Idle and short sequences at the head of the batch (their table rows end, or
+    are stale, before the shared tokens do) do not carry the prefix."""
+    q, k, v, tables, lens_t, slots, _ = decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype, seed=8)
+    order = sorted(range(len(lens)), key=lambda b: lens[b])  # the idle and the short first
+    first = next(i for i, b in enumerate(order) if lens[b] >= shared)
+    check_decode(ane, q[order], k, v, tables, lens_t, slots[order], shared, first)
+    bad = slots[order].clone()
+    bad[0] = -1
+    check_decode(ane, q[order], k, v, tables, lens_t, bad, shared, first)
+    # none holds all of them: the longest does, as far as it goes
+    short = lens_t.clone()
+    short[slots] = torch.minimum(short[slots], torch.tensor(shared - 3, device="cuda", dtype=torch.int32))
+    top = max(min(n, shared - 3) for n in lens)
+    first = next(i for i, b in enumerate(order) if min(lens[b], shared - 3) == top)
+    check_decode(ane, q[order], k, v, tables, short, slots[order], shared, first)

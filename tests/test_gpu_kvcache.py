@@ -309,3 +309,22 @@ def test_write_leaves_rows_outside_cu_alone(ane, src):
             m.k[1, m.tables[s][t // 16], t % 16] = k[cu[i] + j].half()
             m.v[1, m.tables[s][t // 16], t % 16] = v[cu[i] + j].half()
     m.same(c)
+
+
+def test_attend_after_the_first_sequence_left(ane):
+    """Continuations of one prompt, of which the first is freed and its table row
+    left behind by a compaction: the others still attend to the prompt."""
+    c = new_cache(layers=1, pages=40, page=16, heads=2, dim=64, slots=5, max_pages=8)
+    assert c.reserve(i32([4]), i32([70])).tolist() == [1]  # lower pages, to be given up
+    assert c.reserve(i32([0]), i32([90])).tolist() == [1]
+    children = i32([1, 2, 3])
+    assert c.fork(i32([0, 0, 0]), children).tolist() == [1, 1, 1]
+    assert c.reserve(children, i32([5, 9, 30])).tolist() == [1, 1, 1]
+    c.free(i32([4, 1]))
+    c.compact()
+    q = torch.randn(3, 4, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).half()
+    got = c.attend(0, q, children, shared=90, out_dtype=torch.float32)
+    want = c.attend(0, q, children, out_dtype=torch.float32)  # nothing shared: each through its own pages
+    assert (got[0] == 0).all()
+    # rounding of the weights to F16 in both, values of a few units
+    assert (got - want).abs().max() < 2 * 2.0 ** -11 * 4
