@@ -243,6 +243,11 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Pool p, uint32_t layer,
         if (cu[mid] <= t) lo = mid; else hi = mid - 1;
     }
     const int32_t s = slots[lo];
+    if (!granted) {  // (reserve_kernel grants a slot's first request alone)
+        bool again = false;
+        for (uint32_t j = threadIdx.x; j < lo; j += kThreads) again |= slots[j] == s;
+        if (__syncthreads_or(again)) return;
+    }
     if (s < 0 || (uint32_t)s >= p.slots || (granted && !granted[lo])) return;
     const int32_t pos = p.lens[s] - (cu ? cu[lo + 1] - t : 1);
     if (pos < 0 || (uint32_t)pos / p.page_tokens >= p.max_pages) return;

@@ -328,3 +328,29 @@ def test_attend_after_the_first_sequence_left(ane):
     assert (got[0] == 0).all()
     # rounding of the weights to F16 in both, values of a few units
     assert (got - want).abs().max() < 2 * 2.0 ** -11 * 4
+
+
+def test_write_takes_a_slot_once(ane):
+    """A slot named twice counts once, the first time, also without granted."""
+    c = new_cache(layers=1, pages=20, page=16, heads=2, dim=64, slots=600, max_pages=3)
+    m = Model(c)
+    assert c.reserve(i32([0, 1, 2]), i32([20, 10, 33])).tolist() == m.reserve([0, 1, 2], [20, 10, 33])
+    rows = torch.randn(600, 4, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).half()
+    k, v = rows[:, :2], rows[:, 2:]
+
+    def wrote(s, back, r):  # row r is the token `back` before the slot's end
+        t = m.lens[s] - back
+        m.k[0, m.tables[s][t // 16], t % 16], m.v[0, m.tables[s][t // 16], t % 16] = k[r], v[r]
+
+    slots = [2, 0, 2, -1, 0, 600] + [5] * 594
+    slots[590] = 1  # far behind its block's own first look
+    slots[599] = 1
+    c.write(0, i32(slots), k, v)
+    for s, r in ((2, 0), (0, 1), (1, 590)):
+        wrote(s, 1, r)
+    m.same(c)
+    c.write(0, i32([1, 0, 1]), k[10:21], v[10:21], cu=i32([0, 3, 4, 11]))
+    for i in range(3):
+        wrote(1, 3 - i, 10 + i)
+    wrote(0, 1, 13)
+    m.same(c)
