@@ -562,11 +562,18 @@ def _stream_of(stream, t) -> int:
     return _Bound.raw_stream(device) if stream is None else stream.cuda_stream
 
 
-def _rows(name: str, t, heads=None, dim=None):
+def _device(t) -> int:
+    """The CUDA device that holds t, as the checks below want it (get_device() of
+    every tensor); -2, which is no tensor's, for one in host memory."""
+    device = t.get_device()
+    return device if device >= 0 else -2
+
+
+def _rows(name: str, t, device: int, heads=None, dim=None):
     """ane_rows of a CUDA tensor [tokens, heads, dim] whose last dimension is
     contiguous."""
-    if t.dim() != 3 or not t.is_cuda:
-        raise ValueError("%s must be a CUDA tensor [tokens, heads, dim]" % name)
+    if t.dim() != 3 or t.get_device() != device:
+        raise ValueError("%s must be a CUDA tensor [tokens, heads, dim] on the call's device" % name)
     st, sh, sd = t.stride()
     if heads is not None and t.shape[1:] != (heads, dim):
         raise ValueError("%s has heads x dim %s, expected %d x %d" % (name, tuple(t.shape[1:]), heads, dim))
@@ -575,9 +582,9 @@ def _rows(name: str, t, heads=None, dim=None):
     return _pack_rows(t.data_ptr(), st, sh)
 
 
-def _i32_vector(name: str, t, n=None) -> int:
-    if t.dtype is not _bound().i32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous int32 CUDA vector" % name)
+def _i32_vector(name: str, t, device: int, n=None) -> int:
+    if t.dtype is not _bound().i32 or t.get_device() != device or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous int32 CUDA vector on the call's device" % name)
     if n is not None and t.numel() != n:
         raise ValueError("%s has %d entries, expected %d" % (name, t.numel(), n))
     return t.data_ptr()
@@ -595,12 +602,19 @@ def _output(out, like, out_dtype, stream):
     return out
 
 
-def _lse_ptr(lse, q):
+def _lse_ptr(lse, q, device: int):
     if lse is None:
         return None
-    if lse.dtype is not _bound().f32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or not lse.is_cuda:
-        raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, heads]")
+    if lse.dtype is not _bound().f32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.get_device() != device:
+        raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, heads] on q's device")
     return lse.data_ptr()
+
+
+def _workspace(t, device: int):
+    """Address and bytes."""
+    if t.get_device() != device or not t.is_contiguous():
+        raise ValueError("workspace must be a contiguous CUDA tensor on q's device")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 @functools.lru_cache(maxsize=1024)
@@ -615,8 +629,8 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     cu_k[s]:cu_k[s+1] of k and v (int32; cu_k defaults to cu_q).  The last query
     of a sequence sees its last key.  scale defaults to dim ** -0.5; out_dtype
     may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp.
-    workspace: a uint8 tensor of ane_attn_prompt_workspace_size bytes (default: a
-    new one where the call needs any)."""
+    workspace: a contiguous tensor of ane_attn_prompt_workspace_size bytes
+    (default: a new one where the call needs any)."""
     T, heads, dim = q.shape
     Tk, kv_heads, _ = k.shape
     if v.shape != k.shape or k.dtype is not q.dtype or v.dtype is not q.dtype:
@@ -626,7 +640,8 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
         raise ValueError("cu_q needs n_seq + 1 entries")
     if cu_k is None and Tk != T:
         raise ValueError("without cu_k, k and v must have as many rows as q")
-    rq, rk, rv = _rows("q", q), _rows("k", k, kv_heads, dim), _rows("v", v)
+    dev = _device(q)
+    rq, rk, rv = _rows("q", q, dev), _rows("k", k, dev, kv_heads, dim), _rows("v", v, dev)
     out = _output(out, q, out_dtype, stream)
     ws_ptr, ws_bytes = None, 0
     if workspace is None:
@@ -636,11 +651,11 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
             if stream is not None:
                 workspace.record_stream(stream)
     if workspace is not None:
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
+        ws_ptr, ws_bytes = _workspace(workspace, dev)
     check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, Tk,
-                                   dim ** -0.5 if scale is None else scale, rq, rk, rv, _i32_vector("cu_q", cu_q),
-                                   None if cu_k is None else _i32_vector("cu_k", cu_k, n_seq + 1), _dtype(out),
-                                   _rows("out", out), _lse_ptr(lse, q), ws_ptr, ws_bytes, _stream_of(stream, q)))
+                                   dim ** -0.5 if scale is None else scale, rq, rk, rv, _i32_vector("cu_q", cu_q, dev),
+                                   None if cu_k is None else _i32_vector("cu_k", cu_k, dev, n_seq + 1), _dtype(out),
+                                   _rows("out", out, dev), _lse_ptr(lse, q, dev), ws_ptr, ws_bytes, _stream_of(stream, q)))
     return out
 
 
@@ -663,22 +678,24 @@ def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, 
     sp, st, sh, sd = strides = k.stride()
     if v.shape != k.shape or v.stride() != strides or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError("k and v must be [pages, page_tokens, kv_heads, dim] of one layout and q's dtype")
-    if kd != dim or (sd != 1 and dim > 1) or not k.is_cuda or not v.is_cuda:
-        raise ValueError("k and v must be CUDA tensors of q's dim, contiguous in it")
-    if tables.dim() != 2 or tables.dtype is not _torch().int32 or not tables.is_cuda or not tables.is_contiguous():
-        raise ValueError("tables must be a contiguous int32 CUDA tensor [n_slots, max_pages]")
+    dev = _device(q)
+    if kd != dim or (sd != 1 and dim > 1) or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k and v must be CUDA tensors of q's dim, contiguous in it, on q's device")
+    if tables.dim() != 2 or tables.dtype is not _torch().int32 or tables.get_device() != dev or not tables.is_contiguous():
+        raise ValueError("tables must be a contiguous int32 CUDA tensor [n_slots, max_pages] on q's device")
     n_slots, max_pages = tables.shape
-    rq = _rows("q", q)
+    rq = _rows("q", q, dev)
     if workspace is None:
         workspace = attn_decode_workspace(B, heads, kv_heads, dim, q.device)
         if stream is not None:
             workspace.record_stream(stream)
     out = _output(out, q, out_dtype, stream)
+    ws_ptr, ws_bytes = _workspace(workspace, dev)
     pg = _pack_pages(k.data_ptr(), v.data_ptr(), pages, page_tokens, sp, st, sh)
     check(_lib.ane_attn_decode_dev(_dtype(q), B, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale,
                                    rq, pg, tables.data_ptr(), n_slots, max_pages,
-                                   _i32_vector("lens", lens, n_slots),
-                                   None if slots is None else _i32_vector("slots", slots, B), shared, _dtype(out),
-                                   _rows("out", out), _lse_ptr(lse, q), workspace.data_ptr(), workspace.numel(),
+                                   _i32_vector("lens", lens, dev, n_slots),
+                                   None if slots is None else _i32_vector("slots", slots, dev, B), shared, _dtype(out),
+                                   _rows("out", out, dev), _lse_ptr(lse, q, dev), ws_ptr, ws_bytes,
                                    _stream_of(stream, q)))
     return out

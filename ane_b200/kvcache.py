@@ -54,6 +54,7 @@ class KVCache:
                            refs.data_ptr(), tables.data_ptr(), lens.data_ptr(), self.slots, self.max_pages,
                            self._ctl.data_ptr())
         self._ref = ctypes.byref(self._desc)
+        self._device = ane._device(k)
 
     @classmethod
     def empty(cls, layers: int, pages: int, page_tokens: int, kv_heads: int, dim: int, slots: int, max_pages: int,
@@ -75,9 +76,9 @@ class KVCache:
         """Grows slots[i] by counts[i] tokens; returns granted (int32, 1 or 0)."""
         n = slots.numel()
         granted = self._granted(granted, n, stream)
-        ane.check(ane.lib.ane_kv_reserve_dev(self._ref, n, ane._i32_vector("slots", slots),
-                                             ane._i32_vector("counts", counts, n),
-                                             ane._i32_vector("granted", granted, n), ane._stream_of(stream, self.k)))
+        ane.check(ane.lib.ane_kv_reserve_dev(self._ref, n, ane._i32_vector("slots", slots, self._device),
+                                             ane._i32_vector("counts", counts, self._device, n),
+                                             ane._i32_vector("granted", granted, self._device, n), ane._stream_of(stream, self.k)))
         return granted
 
     def write(self, layer: int, slots, k, v, cu=None, granted=None, stream=None) -> None:
@@ -85,12 +86,13 @@ class KVCache:
         cache's type; cu None: one row per slot) become the last tokens of
         slots[i] on `layer`; rows of requests that were not granted are dropped."""
         n = slots.numel()
-        rk, rv = ane._rows("k", k, self.kv_heads, self.dim), ane._rows("v", v, self.kv_heads, self.dim)
+        dev = self._device
+        rk, rv = ane._rows("k", k, dev, self.kv_heads, self.dim), ane._rows("v", v, dev, self.kv_heads, self.dim)
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have one shape and dtype")
-        ane.check(ane.lib.ane_kv_write_dev(self._ref, layer, n, ane._i32_vector("slots", slots),
-                                           None if cu is None else ane._i32_vector("cu", cu, n + 1),
-                                           None if granted is None else ane._i32_vector("granted", granted, n),
+        ane.check(ane.lib.ane_kv_write_dev(self._ref, layer, n, ane._i32_vector("slots", slots, dev),
+                                           None if cu is None else ane._i32_vector("cu", cu, dev, n + 1),
+                                           None if granted is None else ane._i32_vector("granted", granted, dev, n),
                                            k.shape[0], ane._dtype(k), rk, rv,
                                            ane._stream_of(stream, self.k)))
 
@@ -98,23 +100,25 @@ class KVCache:
         """children[i] (empty slots) become copies of parents[i]; returns granted."""
         n = children.numel()
         granted = self._granted(granted, n, stream)
-        ane.check(ane.lib.ane_kv_fork_dev(self._ref, n, ane._i32_vector("parents", parents, n),
-                                          ane._i32_vector("children", children),
-                                          ane._i32_vector("granted", granted, n), ane._stream_of(stream, self.k)))
+        ane.check(ane.lib.ane_kv_fork_dev(self._ref, n, ane._i32_vector("parents", parents, self._device, n),
+                                          ane._i32_vector("children", children, self._device),
+                                          ane._i32_vector("granted", granted, self._device, n), ane._stream_of(stream, self.k)))
         return granted
 
     def free(self, slots, stream=None) -> None:
         """The slots give up their pages and are empty."""
-        ane.check(ane.lib.ane_kv_free_dev(self._ref, slots.numel(), ane._i32_vector("slots", slots),
+        ane.check(ane.lib.ane_kv_free_dev(self._ref, slots.numel(), ane._i32_vector("slots", slots, self._device),
                                           ane._stream_of(stream, self.k)))
 
     def copy_pages(self, src, dst, into: "KVCache | None" = None, stream=None) -> None:
         """Pages src[i] to pages dst[i] on all layers (of `into`, or of this
         cache); refs and tables are the caller's."""
         to = self if into is None else into
+        if to._device != self._device:
+            raise ValueError("the caches are on two devices")
         n = src.numel()
-        ane.check(ane.lib.ane_kv_copy_pages_dev(self._ref, to._ref, n, ane._i32_vector("src", src),
-                                                ane._i32_vector("dst", dst, n), ane._stream_of(stream, self.k)))
+        ane.check(ane.lib.ane_kv_copy_pages_dev(self._ref, to._ref, n, ane._i32_vector("src", src, self._device),
+                                                ane._i32_vector("dst", dst, self._device, n), ane._stream_of(stream, self.k)))
 
     def compact(self, refs_out=None, tables_out=None, remap=None, live=None, stream=None):
         """Moves the pages in use to the lowest numbers.  Returns (live, remap):
@@ -130,11 +134,13 @@ class KVCache:
                     t.record_stream(stream)
         refs_out = self.refs if refs_out is None else refs_out
         tables_out = self.tables if tables_out is None else tables_out
-        if tables_out.shape != self.tables.shape or not tables_out.is_contiguous() or tables_out.dtype != torch.int32:
-            raise ValueError("tables_out must be a contiguous int32 tensor of the tables' shape")
-        ane.check(ane.lib.ane_kv_compact_dev(self._ref, ane._i32_vector("refs_out", refs_out, self.pages),
-                                             tables_out.data_ptr(), ane._i32_vector("remap", remap, self.pages),
-                                             ane._i32_vector("live", live, 1), ane._stream_of(stream, self.k)))
+        dev = self._device
+        if (tables_out.shape != self.tables.shape or not tables_out.is_contiguous() or tables_out.dtype != torch.int32 or
+                tables_out.get_device() != dev):
+            raise ValueError("tables_out must be a contiguous int32 CUDA tensor of the tables' shape on their device")
+        ane.check(ane.lib.ane_kv_compact_dev(self._ref, ane._i32_vector("refs_out", refs_out, dev, self.pages),
+                                             tables_out.data_ptr(), ane._i32_vector("remap", remap, dev, self.pages),
+                                             ane._i32_vector("live", live, dev, 1), ane._stream_of(stream, self.k)))
         return live, remap
 
     def attend(self, layer: int, q, slots=None, shared: int = 0, **kw):

@@ -153,3 +153,112 @@ def test_python_refusals():
             KVCache(*args)
     with pytest.raises(TypeError):
         KVCache(k.float(), k.float(), ints(4), ints(2, 3), ints(2))
+
+
+class OnDevice:
+    """A tensor as the bindings see it, said to be on CUDA device `device` (-1: the host)."""
+
+    def __init__(self, t, device=0):
+        self._t, self._device = t, device
+
+    is_cuda = property(lambda self: self._device >= 0)
+
+    def get_device(self):
+        return self._device
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The calls that would reach the device; none is made."""
+    made = []
+    for name in ("ane_attn_prompt_dev", "ane_attn_decode_dev", "ane_kv_reserve_dev", "ane_kv_write_dev", "ane_kv_fork_dev",
+                 "ane_kv_free_dev", "ane_kv_copy_pages_dev", "ane_kv_compact_dev"):
+        monkeypatch.setattr(L, name, lambda *args, name=name: made.append(name) or 0)
+    monkeypatch.setattr(ane, "_stream_of", lambda stream, t: 0)
+    return made
+
+
+WHERE = [-1, 1]  # on the host, on another device
+
+
+def half(*shape):
+    return OnDevice(torch.zeros(shape, dtype=torch.float16))
+
+
+def ints(*shape):
+    return OnDevice(torch.zeros(shape, dtype=torch.int32))
+
+
+def moved(args, name, device):
+    args = dict(args)
+    if name:
+        args[name] = OnDevice(args[name]._t, device)
+    return args
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_prompt_takes_nothing_from_elsewhere(launches, device):
+    """A pointer to host memory, or to another device's, never reaches a kernel."""
+    n = ane.lib.ane_attn_prompt_workspace_size(1, 4, 2, 64, 64, 2048)
+    args = dict(q=half(64, 4, 64), k=half(2048, 2, 64), v=half(2048, 2, 64), cu_q=ints(2), cu_k=ints(2),
+                out=half(64, 4, 64), lse=OnDevice(torch.zeros(64, 4)), workspace=OnDevice(torch.zeros(n, dtype=torch.uint8)))
+    assert n > 0
+    ane.attn_prompt(**args)
+    assert launches == ["ane_attn_prompt_dev"]
+    for name in args:
+        with pytest.raises(ValueError):
+            ane.attn_prompt(**moved(args, name, device))
+    with pytest.raises(ValueError):
+        ane.attn_prompt(**{**args, "workspace": OnDevice(torch.zeros(2 * n, dtype=torch.uint8)[::2])})
+    assert len(launches) == 1
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_decode_takes_nothing_from_elsewhere(launches, device):
+    n = ane.lib.ane_attn_decode_workspace_size(2, 4, 2, 64)
+    args = dict(q=half(2, 4, 64), k=half(8, 16, 2, 64), v=half(8, 16, 2, 64), tables=ints(3, 4), lens=ints(3),
+                slots=ints(2), out=half(2, 4, 64), lse=OnDevice(torch.zeros(2, 4)),
+                workspace=OnDevice(torch.zeros(n, dtype=torch.uint8)))
+    ane.attn_decode(**args)
+    assert launches == ["ane_attn_decode_dev"]
+    for name in args:
+        with pytest.raises(ValueError):
+            ane.attn_decode(**moved(args, name, device))
+    assert len(launches) == 1
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_cache_takes_nothing_from_elsewhere(launches, device):
+    from ane_b200.kvcache import KVCache
+
+    def new(d=0):
+        pool = OnDevice(torch.zeros(2, 8, 16, 2, 64, dtype=torch.float16), d)
+        return KVCache(pool, pool, ints(8), ints(3, 4), ints(3))
+
+    c = new()
+    calls = [
+        (c.reserve, dict(slots=ints(1), counts=ints(1), granted=ints(1))),
+        (c.write, dict(layer=0, slots=ints(1), k=half(1, 2, 64), v=half(1, 2, 64), cu=ints(2), granted=ints(1))),
+        (c.fork, dict(parents=ints(1), children=ints(1), granted=ints(1))),
+        (c.free, dict(slots=ints(1))),
+        (c.copy_pages, dict(src=ints(2), dst=ints(2))),
+        (c.compact, dict(refs_out=ints(8), tables_out=ints(3, 4), remap=ints(8), live=ints(1))),
+    ]
+    for call, args in calls:
+        call(**args)
+    made = len(launches)
+    assert made == len(calls)
+    for call, args in calls:
+        for name in args:
+            if name != "layer":
+                with pytest.raises(ValueError):
+                    call(**moved(args, name, device))
+    with pytest.raises(ValueError):
+        c.copy_pages(ints(1), ints(1), into=new(device))
+    host = new(-1)
+    with pytest.raises(ValueError):
+        host.free(OnDevice(torch.zeros(1, dtype=torch.int32), -1))
+    assert len(launches) == made
