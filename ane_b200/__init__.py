@@ -590,13 +590,28 @@ def _i32_vector(name: str, t, device: int, n=None) -> int:
     return t.data_ptr()
 
 
+def _made_for(stream, make, returned=True):
+    """A new tensor, make(), for a call on `stream` (None: the current one), from
+    that stream's memory: a block that the current stream gave up may still be in
+    use there by work that `stream` does not wait for.  One that is returned to the
+    caller is kept until the current stream is done with it."""
+    if stream is None:
+        return make()
+    torch = _torch()
+    with torch.cuda.stream(stream):
+        t = make()
+    if returned:
+        t.record_stream(torch.cuda.current_stream(t.device))
+    return t
+
+
 def _output(out, like, out_dtype, stream):
-    """`out` or a new tensor of like's shape; a new one is kept alive for `stream`."""
+    """`out` or a new tensor of like's shape."""
     if out is None:
+        if stream is not None:
+            return _made_for(stream, lambda: _output(None, like, out_dtype, None))
         # (1.5 us of the host; torch.empty with the shape, dtype and device spelt out 3.4)
         out = _bound().empty_like(like, dtype=out_dtype, memory_format=_Bound.contiguous)
-        if stream is not None:
-            out.record_stream(stream)
     elif out.shape != like.shape:
         raise ValueError("out must have the shape of q")
     return out
@@ -614,7 +629,7 @@ def _workspace(t, device: int):
     """Address and bytes."""
     if t.get_device() != device or not t.is_contiguous():
         raise ValueError("workspace must be a contiguous CUDA tensor on q's device")
-    return t.data_ptr(), t.numel() * t.element_size()
+    return t.data_ptr(), t.nbytes
 
 
 @functools.lru_cache(maxsize=1024)
@@ -647,9 +662,7 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     if workspace is None:
         ws_bytes = _prompt_workspace_size(n_seq, heads, kv_heads, dim, T, Tk)
         if ws_bytes:
-            workspace = q.new_empty(ws_bytes, dtype=_torch().uint8)
-            if stream is not None:
-                workspace.record_stream(stream)
+            workspace = _made_for(stream, lambda: q.new_empty(ws_bytes, dtype=_torch().uint8), returned=False)
     if workspace is not None:
         ws_ptr, ws_bytes = _workspace(workspace, dev)
     check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, Tk,
@@ -681,14 +694,12 @@ def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, 
     dev = _device(q)
     if kd != dim or (sd != 1 and dim > 1) or k.get_device() != dev or v.get_device() != dev:
         raise ValueError("k and v must be CUDA tensors of q's dim, contiguous in it, on q's device")
-    if tables.dim() != 2 or tables.dtype is not _torch().int32 or tables.get_device() != dev or not tables.is_contiguous():
+    if tables.dim() != 2 or tables.dtype is not _bound().i32 or tables.get_device() != dev or not tables.is_contiguous():
         raise ValueError("tables must be a contiguous int32 CUDA tensor [n_slots, max_pages] on q's device")
     n_slots, max_pages = tables.shape
     rq = _rows("q", q, dev)
     if workspace is None:
-        workspace = attn_decode_workspace(B, heads, kv_heads, dim, q.device)
-        if stream is not None:
-            workspace.record_stream(stream)
+        workspace = _made_for(stream, lambda: attn_decode_workspace(B, heads, kv_heads, dim, q.device), returned=False)
     out = _output(out, q, out_dtype, stream)
     ws_ptr, ws_bytes = _workspace(workspace, dev)
     pg = _pack_pages(k.data_ptr(), v.data_ptr(), pages, page_tokens, sp, st, sh)

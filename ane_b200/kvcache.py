@@ -67,10 +67,11 @@ class KVCache:
 
     def _granted(self, granted, n, stream):
         if granted is None:
-            granted = torch.empty(n, dtype=torch.int32, device=self.k.device)
-            if stream is not None:
-                granted.record_stream(stream)
+            granted = self._new(n, stream)
         return granted
+
+    def _new(self, n, stream):
+        return ane._made_for(stream, lambda: torch.empty(n, dtype=torch.int32, device=self.k.device))
 
     def reserve(self, slots, counts, granted=None, stream=None):
         """Grows slots[i] by counts[i] tokens; returns granted (int32, 1 or 0)."""
@@ -125,13 +126,8 @@ class KVCache:
         the number of pages in use (int32 [1]) and each page's new number (-1:
         free).  refs_out and tables_out default to the cache's own arrays; given
         others, the cache keeps its old state, whose pages stay intact."""
-        new = lambda t, n: torch.empty(n, dtype=torch.int32, device=self.k.device) if t is None else t  # noqa: E731
-        given = (remap, live)
-        remap, live = new(remap, self.pages), new(live, 1)
-        if stream is not None:
-            for g, t in zip(given, (remap, live)):
-                if g is None:
-                    t.record_stream(stream)
+        remap = self._new(self.pages, stream) if remap is None else remap
+        live = self._new(1, stream) if live is None else live
         refs_out = self.refs if refs_out is None else refs_out
         tables_out = self.tables if tables_out is None else tables_out
         dev = self._device

@@ -468,3 +468,36 @@ def test_decode_prefix_of_a_row_that_holds_it(ane, lens, shared, heads, kv_heads
     top = max(min(n, shared - 3) for n in lens)
     first = next(i for i, b in enumerate(order) if min(lens[b], shared - 3) == top)
     check_decode(ane, q[order], k, v, tables, short, slots[order], shared, first)
+
+
+def give_up_busy(*sizes):
+    """Blocks of the current stream's memory, freed while the work that writes them
+    still waits there."""
+    held = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes]
+    torch.cuda._sleep(100_000_000)  # about 50 ms
+    for h in held:
+        h.fill_(0xff)
+
+
+@pytest.mark.parametrize("lq,lk", [([200, 64], [200, 64]), ([100, 60], [3000, 2000])])
+def test_prompt_on_a_side_stream_next_to_freed_memory(ane, lq, lk):
+    q, k, v, cq, ck, out = prompt_case(ane, lq, lk, 4, 2, 128, F16, seed=9)
+    c, d, side = i32(cq), i32(ck), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ws = ane.lib.ane_attn_prompt_workspace_size(2, 4, 2, 128, q.shape[0], k.shape[0])
+    give_up_busy(q.numel() * 2, max(ws, 1))
+    got = ane.attn_prompt(q, k, v, c, d, stream=side)
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(got[cq[0]:cq[-1]], out[cq[0]:cq[-1]])
+
+
+def test_decode_on_a_side_stream_next_to_freed_memory(ane):
+    q, k, v, tables, lens, slots, out = decode_case(ane, [1500, 0, 1301, 1290], 1290, 8, 2, 128, 64, BF16)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    give_up_busy(q.numel() * 2, ane.attn_decode_workspace(4, 8, 2, 128).numel())
+    got = ane.attn_decode(q, k, v, tables, lens, slots=slots, shared=1290, stream=side)
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(got, out)

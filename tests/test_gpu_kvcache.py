@@ -354,3 +354,25 @@ def test_write_takes_a_slot_once(ane):
         wrote(1, 3 - i, 10 + i)
     wrote(0, 1, 13)
     m.same(c)
+
+
+def test_side_stream_next_to_freed_memory(ane):
+    """What the cache's calls return does not lie in memory that work on the current
+    stream is still to write."""
+    c = new_cache(pages=40)
+    m = Model(c)
+    one, ten, two = i32([1]), i32([10]), i32([2])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    held = [torch.empty(n, dtype=torch.int32, device="cuda") for n in (1, 1, 1, 40)]
+    torch.cuda._sleep(100_000_000)  # about 50 ms
+    for h in held:
+        h.fill_(-5)
+    del held, h
+    got = [c.reserve(one, ten, stream=side), c.fork(one, two, stream=side), *c.compact(stream=side)]
+    side.synchronize()
+    torch.cuda.synchronize()
+    want = [m.reserve([1], [10]), m.fork([1], [2])]
+    live, remap = m.compact()
+    assert [g.tolist() for g in got] == want + [[live], remap]
+    m.same(c)
