@@ -31,6 +31,12 @@ constexpr uint32_t kBigBlocks = 148;   // of prefix_kernel, about
 constexpr int kTile = 64;              // tokens per key/value tile
 constexpr int kThreads = 192;          // four computing warps, the producers of K and of V
 constexpr int kJoinThreads = 128;
+// Up to so many sequences join_kernel counts the own tiles itself, which hides behind
+// the last blocks of decode_kernel but costs each of its blocks a pass over the batch;
+// above, it reads decode_kernel's counts.  32/8 heads, 600 tokens each, us counted and
+// read: 24 sequences 20.7 and 22.8, 64 43.2 and 45.2, 96 58 and 58, 128 75 and 72, 256
+// 157 and 128, 1024 1208 and 457.
+constexpr uint32_t kCountedBatch = 96;
 constexpr uint32_t kKept = 256;        // sequences whose slot and length stay in shared memory
 constexpr int kPagesAhead = 4;         // tiles whose page numbers are read ahead
 constexpr int kUnits = 4;              // units announced ahead
@@ -54,6 +60,7 @@ struct Params {
     ane_rows q, out;
     const int32_t *tables, *lens, *slots;
     float* lse;
+    int32_t* cum;       // [batch + 1] own tiles of the sequences before b, for join_kernel (NULL: it counts them)
     float *po, *pm;     // prefix_kernel's partials: rows x dim; rows x {m, l}
     float *so, *sm;     // decode_kernel's
     int* err;
@@ -362,6 +369,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();
     const int per_g = (int)(p.kv_heads * p.subs);  // units of a group
+    if (p.cum && blockIdx.x == 0)
+        for (uint32_t b = threadIdx.x; b <= p.batch; b += kThreads) p.cum[b] = sm.cum[b];
     const int total = group_start(p, sm.cum, p.groups) * per_g;
     const int per = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
 
@@ -773,24 +782,31 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const size_t prow = (size_t)h * all_rows + b * p.group + g, pstep = all_rows * p.kv_heads;
     const uint32_t grp = b / p.per_unit, sub = p.group > 16 ? g / 16 : 0;
     const uint32_t row = p.group > 16 ? g % 16 : b % p.per_unit * p.group + g;
-    // Where decode_kernel's blocks cut the line, from the lengths, while they end:
-    // own tiles of the sequences before the row's unit, of the unit and of all.
+    // Where decode_kernel's blocks cut the line: own tiles of the sequences before the
+    // row's unit, of the unit and of all.
     int tiles[3] = {0, 0, 0};
-    for (uint32_t x = threadIdx.x; x < p.batch; x += kJoinThreads) {
-        const int own = own_tiles(p, len_of(p, x)), u = (int)(x / p.per_unit) - (int)grp;
-        tiles[0] += u < 0 ? own : 0;
-        tiles[1] += u == 0 ? own : 0;
-        tiles[2] += own;
-    }
+    if (p.cum) {
+        ptx::griddep_wait();
+        tiles[0] = __ldcg(p.cum + grp * p.per_unit);
+        tiles[1] = __ldcg(p.cum + min((grp + 1) * p.per_unit, p.batch)) - tiles[0];
+        tiles[2] = __ldcg(p.cum + p.batch);
+    } else {  // from the lengths, while those blocks end
+        for (uint32_t x = threadIdx.x; x < p.batch; x += kJoinThreads) {
+            const int own = own_tiles(p, len_of(p, x)), u = (int)(x / p.per_unit) - (int)grp;
+            tiles[0] += u < 0 ? own : 0;
+            tiles[1] += u == 0 ? own : 0;
+            tiles[2] += own;
+        }
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
-        tiles[i] = __reduce_add_sync(0xffffffffu, tiles[i]);
-        if (lane == 0) sm_tiles[warp][i] = tiles[i];
-    }
-    __syncthreads();
+        for (int i = 0; i < 3; i++) {
+            tiles[i] = __reduce_add_sync(0xffffffffu, tiles[i]);
+            if (lane == 0) sm_tiles[warp][i] = tiles[i];
+        }
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 3; i++) tiles[i] = sm_tiles[0][i] + sm_tiles[1][i] + sm_tiles[2][i] + sm_tiles[3][i];
-    ptx::griddep_wait();
+        for (int i = 0; i < 3; i++) tiles[i] = sm_tiles[0][i] + sm_tiles[1][i] + sm_tiles[2][i] + sm_tiles[3][i];
+        ptx::griddep_wait();
+    }
     const int per_g = (int)(p.kv_heads * p.subs), id = (int)(h * p.subs + sub), c0 = tiles[0];
     const int total = ((int)(p.groups * (kUnitCost + p.prefix_tiles)) + tiles[2]) * per_g;
     const int per = (int)(((unsigned)total + p.blocks - 1) / p.blocks);
@@ -862,7 +878,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
 // ------------------------------------------------------------------ launch
 struct Layout {
     uint32_t per_unit, groups, subs, rows, pairs, big_splits;
-    size_t pm, po, sm, so, bytes;
+    size_t cum, pm, po, sm, so, bytes;
 };
 Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
     Layout l;
@@ -882,6 +898,7 @@ Layout layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
         at += round_up(bytes, 256);
         return here;
     };
+    l.cum = take((batch + 1) * 4);
     l.pm = take(prefix_rows * 8);
     l.sm = take(own_rows * 8);
     l.po = take(prefix_rows * dim * 4);
@@ -975,6 +992,7 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.scale2 = scale * attn::kLog2e;
     p.q = *q, p.out = *out;
     p.tables = tables, p.lens = lens, p.slots = slots, p.lse = lse;
+    if (batch > kCountedBatch) p.cum = reinterpret_cast<int32_t*>(ws + l.cum);
     p.pm = reinterpret_cast<float*>(ws + l.pm), p.po = reinterpret_cast<float*>(ws + l.po);
     p.sm = reinterpret_cast<float*>(ws + l.sm), p.so = reinterpret_cast<float*>(ws + l.so);
     p.err = device_timeout_flag();

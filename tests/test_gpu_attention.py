@@ -501,3 +501,18 @@ def test_decode_on_a_side_stream_next_to_freed_memory(ane):
     side.synchronize()
     torch.cuda.synchronize()
     assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("batch", [95, 96, 97, 400])
+def test_decode_joins_of_many_sequences(ane, batch):
+    """Parts of many sequences, however their tables are wide and whatever the
+    workspace holds."""
+    lens = [(61 * b) % 190 + 20 for b in range(batch)]
+    lens[1] = 1500
+    q, k, v, tables, lens_t, slots, out = decode_case(ane, lens, 20, 4, 2, 64, 16, F16, seed=7)
+    ws = ane.attn_decode_workspace(batch, 4, 2, 64)
+    wide = torch.nn.functional.pad(tables, (0, 3000), value=10 ** 9).contiguous()
+    for table in (tables, wide):
+        ws.random_(0, 255)
+        got = ane.attn_decode(q, k, v, table, lens_t, slots=slots, shared=20, workspace=ws)
+        assert torch.equal(got, out)
