@@ -502,12 +502,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (following.head >= 0) af = begin(following);
         };
         while (ok && u.head >= 0) {
-            if (u.t1 <= u.t0) look_ahead();
-            int t = u.t0;
-            while (ok && t < u.t1) {
+            int t = u.t0, stop = min(u.t0 + S::kStages, u.t1);
+            for (;;) {
 #pragma unroll
                 for (int d = 0; d < kPagesAhead; d++) {  // (page numbers on their way cannot change registers)
-                    if (!ok || t >= u.t1) continue;
+                    if (!ok || t >= stop || ((t - u.t0) & (kPagesAhead - 1)) != d) continue;
                     const Tile now = a.load.t;
                     const int page = a.page[d];
                     if (t + 1 < u.t1) advance(a.load, u);
@@ -526,11 +525,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                         tma_load_4d(sm.kv[st][is_v] + half * S::kHalf + key0 * 128, map, &sm.full[st],
                                     half * 64, u.head, j & ((1 << p.page_shift) - 1), (uint32_t)page < p.pages ? page : 0);
                     if (t + kPagesAhead < u.t1) advance(a.read, u), a.page[d] = entry(a.read);
-                    // with the first tiles on their way
-                    if (t == min(u.t0 + S::kStages, u.t1) - 1) look_ahead();
                     t++;
                     n++;
                 }
+                if (!ok) break;
+                // with the first tiles on their way (in one place: its code is long)
+                if (t == min(u.t0 + S::kStages, u.t1)) look_ahead(), stop = u.t1;
+                if (t >= u.t1) break;
             }
             u = following;
             a = af;
