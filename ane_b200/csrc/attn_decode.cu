@@ -771,7 +771,8 @@ __global__ void __launch_bounds__(kBigThreads, 1)
 // One block per output row; its warps take the partial results in turn.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
-    __shared__ float sm_m[4], sm_l[4], sm_o[4][128];
+    __shared__ float sm_m[4], sm_l[4];
+    __shared__ float4 sm_o[4][32];
     __shared__ int sm_tiles[4][3];
     ptx::griddep_launch_dependents();
     const uint32_t b = blockIdx.x, head = blockIdx.y, h = head / p.group, g = head % p.group;
@@ -852,7 +853,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
         }
     }
     if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
-    *reinterpret_cast<float4*>(&sm_o[warp][lane * 4]) = make_float4(o[0], o[1], o[2], o[3]);
+    sm_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
     __syncthreads();
     const uint32_t c = threadIdx.x;
     m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
@@ -863,7 +864,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     for (int w = 0; w < 4; w++) {
         const float f = exp2_fast(sm_m[w] - base);
         l += sm_l[w] * f;
-        sum += sm_o[w][c] * f;
+        sum += reinterpret_cast<const float*>(sm_o[w])[c] * f;
     }
     if (c < p.dim) {
         const float y = l == 0.0f ? 0.0f : sum / l;
