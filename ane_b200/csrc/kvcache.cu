@@ -498,7 +498,7 @@ int ane_kv_write_dev(const ane_kv_cache* cache, uint32_t layer, uint32_t n, cons
                   "kv_write: rows must be F32 or of the cache's dtype");
     const size_t elem = src_dtype == ANE_DTYPE_F32 ? 4 : 2;
     for (const ane_rows* r : {k, v}) {
-        if (n == 0) break;
+        if (n == 0 || tokens == 0) break;  // (no rows may have no memory)
         ANE_ARG_CHECK(r->data && (uintptr_t)r->data % 16 == 0 && r->token_stride * elem % 16 == 0 &&
                           r->head_stride * elem % 16 == 0,
                       "kv_write: rows must be 16-byte aligned with strides of whole 16 bytes");

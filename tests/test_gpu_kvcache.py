@@ -376,3 +376,15 @@ def test_side_stream_next_to_freed_memory(ane):
     live, remap = m.compact()
     assert [g.tolist() for g in got] == want + [[live], remap]
     m.same(c)
+
+
+def test_write_of_no_rows(ane):
+    """Requests without rows, whose tensors have no memory."""
+    c = new_cache()
+    assert c.reserve(i32([0, 1]), i32([3, 0])).tolist() == [1, 1]
+    m = Model(c)
+    none = torch.empty(0, 2, 64, device="cuda")
+    c.write(0, i32([0, 1]), none, none, cu=i32([0, 0, 0]))
+    c.write(0, i32([]), none, none)
+    c.write(0, i32([]), none.half(), none.half(), cu=i32([0]))
+    m.same(c)
