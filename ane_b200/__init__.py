@@ -533,7 +533,8 @@ class _Bound:
         cls.i32, cls.f32 = torch.int32, torch.float32
         cls.dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # ANE_DTYPE_*
         cls.empty_like, cls.contiguous = torch.empty_like, torch.contiguous_format
-        cls.current_device = torch.cuda.current_device
+        # (a call has CUDA tensors: CUDA is up, which torch.cuda.current_device checks each time)
+        cls.current_device = staticmethod(getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device)
         # the handle without a Stream object, which costs 3 us
         cls.raw_stream = staticmethod(getattr(torch._C, "_cuda_getCurrentRawStream", None) or
                                       (lambda d: torch.cuda.current_stream(d).cuda_stream))
@@ -553,10 +554,12 @@ def _dtype(t) -> int:
     return code
 
 
-def _stream_of(stream, t) -> int:
-    """The cudaStream_t of `stream`, or of the current stream of t's device, which
-    has to be the current device."""
-    device, current = t.get_device(), _bound().current_device()
+def _stream_of(stream, device: int) -> int:
+    """The cudaStream_t of `stream`, or of the current stream of `device`, which has
+    to be the current device."""
+    if device < 0:
+        raise ValueError("the tensors are not on a CUDA device")
+    current = _bound().current_device()
     if device != current:
         raise ValueError("the tensors are on device %d, the current device is %d" % (device, current))
     return _Bound.raw_stream(device) if stream is None else stream.cuda_stream
@@ -579,7 +582,14 @@ def _rows(name: str, t, device: int, heads=None, dim=None):
         raise ValueError("%s has heads x dim %s, expected %d x %d" % (name, tuple(t.shape[1:]), heads, dim))
     if sd != 1 and t.shape[2] > 1:
         raise ValueError("%s: the last dimension must be contiguous" % name)
+    if (st | sh) & 7 or not st or not sh:  # torch lets the stride of a dimension of one entry be anything
+        n, h, d = t.shape
+        st, sh = st if n != 1 else h * d, sh if h != 1 else d
     return _pack_rows(t.data_ptr(), st, sh)
+
+
+def _layout(t):
+    return [s for s, n in zip(t.stride(), t.shape) if n != 1]
 
 
 def _i32_vector(name: str, t, device: int, n=None) -> int:
@@ -620,7 +630,8 @@ def _output(out, like, out_dtype, stream):
 def _lse_ptr(lse, q, device: int):
     if lse is None:
         return None
-    if lse.dtype is not _bound().f32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.get_device() != device:
+    if (lse.dtype is not _bound().f32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or
+            lse.get_device() != device):
         raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, heads] on q's device")
     return lse.data_ptr()
 
@@ -668,7 +679,8 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     check(_lib.ane_attn_prompt_dev(_dtype(q), n_seq, heads, kv_heads, dim, T, Tk,
                                    dim ** -0.5 if scale is None else scale, rq, rk, rv, _i32_vector("cu_q", cu_q, dev),
                                    None if cu_k is None else _i32_vector("cu_k", cu_k, dev, n_seq + 1), _dtype(out),
-                                   _rows("out", out, dev), _lse_ptr(lse, q, dev), ws_ptr, ws_bytes, _stream_of(stream, q)))
+                                   _rows("out", out, dev), _lse_ptr(lse, q, dev), ws_ptr, ws_bytes,
+                                   _stream_of(stream, dev)))
     return out
 
 
@@ -689,7 +701,8 @@ def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, 
     B, heads, dim = q.shape
     pages, page_tokens, kv_heads, kd = k.shape
     sp, st, sh, sd = strides = k.stride()
-    if v.shape != k.shape or v.stride() != strides or k.dtype is not q.dtype or v.dtype is not q.dtype:
+    if (v.shape != k.shape or (v.stride() != strides and _layout(v) != _layout(k)) or k.dtype is not q.dtype or
+            v.dtype is not q.dtype):
         raise ValueError("k and v must be [pages, page_tokens, kv_heads, dim] of one layout and q's dtype")
     dev = _device(q)
     if kd != dim or (sd != 1 and dim > 1) or k.get_device() != dev or v.get_device() != dev:
@@ -702,11 +715,16 @@ def attn_decode(q, k, v, tables, lens, slots=None, shared: int = 0, scale=None, 
         workspace = _made_for(stream, lambda: attn_decode_workspace(B, heads, kv_heads, dim, q.device), returned=False)
     out = _output(out, q, out_dtype, stream)
     ws_ptr, ws_bytes = _workspace(workspace, dev)
+    # (a dimension of one entry: as in _rows)
+    if pages == 1:
+        sp = page_tokens * kv_heads * dim
+    if kv_heads == 1:
+        sh = dim
     pg = _pack_pages(k.data_ptr(), v.data_ptr(), pages, page_tokens, sp, st, sh)
     check(_lib.ane_attn_decode_dev(_dtype(q), B, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale,
                                    rq, pg, tables.data_ptr(), n_slots, max_pages,
                                    _i32_vector("lens", lens, dev, n_slots),
                                    None if slots is None else _i32_vector("slots", slots, dev, B), shared, _dtype(out),
                                    _rows("out", out, dev), _lse_ptr(lse, q, dev), ws_ptr, ws_bytes,
-                                   _stream_of(stream, q)))
+                                   _stream_of(stream, dev)))
     return out

@@ -75,11 +75,11 @@ class KVCache:
 
     def reserve(self, slots, counts, granted=None, stream=None):
         """Grows slots[i] by counts[i] tokens; returns granted (int32, 1 or 0)."""
-        n = slots.numel()
+        n, dev = slots.numel(), self._device
         granted = self._granted(granted, n, stream)
-        ane.check(ane.lib.ane_kv_reserve_dev(self._ref, n, ane._i32_vector("slots", slots, self._device),
-                                             ane._i32_vector("counts", counts, self._device, n),
-                                             ane._i32_vector("granted", granted, self._device, n), ane._stream_of(stream, self.k)))
+        ane.check(ane.lib.ane_kv_reserve_dev(self._ref, n, ane._i32_vector("slots", slots, dev),
+                                             ane._i32_vector("counts", counts, dev, n),
+                                             ane._i32_vector("granted", granted, dev, n), ane._stream_of(stream, dev)))
         return granted
 
     def write(self, layer: int, slots, k, v, cu=None, granted=None, stream=None) -> None:
@@ -95,31 +95,31 @@ class KVCache:
                                            None if cu is None else ane._i32_vector("cu", cu, dev, n + 1),
                                            None if granted is None else ane._i32_vector("granted", granted, dev, n),
                                            k.shape[0], ane._dtype(k), rk, rv,
-                                           ane._stream_of(stream, self.k)))
+                                           ane._stream_of(stream, dev)))
 
     def fork(self, parents, children, granted=None, stream=None):
         """children[i] (empty slots) become copies of parents[i]; returns granted."""
-        n = children.numel()
+        n, dev = children.numel(), self._device
         granted = self._granted(granted, n, stream)
-        ane.check(ane.lib.ane_kv_fork_dev(self._ref, n, ane._i32_vector("parents", parents, self._device, n),
-                                          ane._i32_vector("children", children, self._device),
-                                          ane._i32_vector("granted", granted, self._device, n), ane._stream_of(stream, self.k)))
+        ane.check(ane.lib.ane_kv_fork_dev(self._ref, n, ane._i32_vector("parents", parents, dev, n),
+                                          ane._i32_vector("children", children, dev),
+                                          ane._i32_vector("granted", granted, dev, n), ane._stream_of(stream, dev)))
         return granted
 
     def free(self, slots, stream=None) -> None:
         """The slots give up their pages and are empty."""
         ane.check(ane.lib.ane_kv_free_dev(self._ref, slots.numel(), ane._i32_vector("slots", slots, self._device),
-                                          ane._stream_of(stream, self.k)))
+                                          ane._stream_of(stream, self._device)))
 
     def copy_pages(self, src, dst, into: "KVCache | None" = None, stream=None) -> None:
         """Pages src[i] to pages dst[i] on all layers (of `into`, or of this
         cache); refs and tables are the caller's."""
         to = self if into is None else into
-        if to._device != self._device:
+        n, dev = src.numel(), self._device
+        if to._device != dev:
             raise ValueError("the caches are on two devices")
-        n = src.numel()
-        ane.check(ane.lib.ane_kv_copy_pages_dev(self._ref, to._ref, n, ane._i32_vector("src", src, self._device),
-                                                ane._i32_vector("dst", dst, self._device, n), ane._stream_of(stream, self.k)))
+        ane.check(ane.lib.ane_kv_copy_pages_dev(self._ref, to._ref, n, ane._i32_vector("src", src, dev),
+                                                ane._i32_vector("dst", dst, dev, n), ane._stream_of(stream, dev)))
 
     def compact(self, refs_out=None, tables_out=None, remap=None, live=None, stream=None):
         """Moves the pages in use to the lowest numbers.  Returns (live, remap):
@@ -131,12 +131,12 @@ class KVCache:
         refs_out = self.refs if refs_out is None else refs_out
         tables_out = self.tables if tables_out is None else tables_out
         dev = self._device
-        if (tables_out.shape != self.tables.shape or not tables_out.is_contiguous() or tables_out.dtype != torch.int32 or
-                tables_out.get_device() != dev):
+        if (tables_out.shape != self.tables.shape or not tables_out.is_contiguous() or
+                tables_out.dtype != torch.int32 or tables_out.get_device() != dev):
             raise ValueError("tables_out must be a contiguous int32 CUDA tensor of the tables' shape on their device")
         ane.check(ane.lib.ane_kv_compact_dev(self._ref, ane._i32_vector("refs_out", refs_out, dev, self.pages),
                                              tables_out.data_ptr(), ane._i32_vector("remap", remap, dev, self.pages),
-                                             ane._i32_vector("live", live, dev, 1), ane._stream_of(stream, self.k)))
+                                             ane._i32_vector("live", live, dev, 1), ane._stream_of(stream, dev)))
         return live, remap
 
     def attend(self, layer: int, q, slots=None, shared: int = 0, **kw):

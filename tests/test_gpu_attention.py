@@ -516,3 +516,20 @@ def test_decode_joins_of_many_sequences(ane, batch):
         ws.random_(0, 255)
         got = ane.attn_decode(q, k, v, table, lens_t, slots=slots, shared=20, workspace=ws)
         assert torch.equal(got, out)
+
+
+def test_single_rows_of_any_stride(ane):
+    """A dimension of one entry may have any stride (torch calls such a tensor
+    contiguous)."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    buf = torch.randn(3, 8 * 64, device="cuda", generator=g).half()
+    odd = lambda i, h: torch.as_strided(buf[i], (1, h, 64), (8 * 64 + 3, 64, 1))  # noqa: E731
+    q, k, v = odd(0, 8), odd(1, 2), odd(2, 2)
+    out = ane.attn_prompt(q, k, v, i32([0, 1]))
+    assert torch.equal(out[0], v[0].repeat_interleave(4, 0))
+    one = lambda i: torch.as_strided(buf[i], (5, 1, 64), (64, 67, 1))  # noqa: E731  (one head)
+    check_rows(ane.attn_prompt(one(0), one(1), one(2), i32([0, 5]))[:, 0], F16, one(0)[:, 0], one(1)[:, 0], one(2)[:, 0],
+               0.125, torch.arange(1, 6, device="cuda"))
+    pool = lambda i: torch.as_strided(buf[i], (1, 8, 1, 64), (515, 64, 67, 1))  # noqa: E731  (one page, one head)
+    out = ane.attn_decode(odd(0, 8), pool(1), pool(2).contiguous().view(1, 8, 1, 64), i32([[0]]), i32([7]))
+    check_rows(out[0], F16, odd(0, 8)[0], pool(1)[0, :7, 0], pool(2)[0, :7, 0], 0.125, torch.full((8,), 7, device="cuda"))
