@@ -947,6 +947,7 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     int rc = attn::check_shapes("attn_decode", dtype, out_dtype, heads, kv_heads, dim, scale);
     if (rc) return rc;
     ANE_ARG_CHECK(batch <= kMaxBatch, "attn_decode: at most 1024 sequences");
+    ANE_ARG_CHECK(heads <= 65535, "attn_decode: at most 65535 heads");  // the join's grid
     ANE_ARG_CHECK(q && pages && tables && lens && out, "attn_decode: NULL pointer");
     ANE_ARG_CHECK(slots || batch <= n_slots, "attn_decode: without slots the batch must not exceed n_slots");
     ANE_ARG_CHECK(n_slots > 0 && max_pages > 0, "attn_decode: empty table");

@@ -460,7 +460,7 @@ typedef struct ane_rows {
  * finite (a key that a query does not see yet has weight 0, and 0 * NaN is NaN).  lse (NULL to skip)
  * receives [total_q][heads] natural logarithms of the softmax sums.
  * scale > 0; dim % 8 == 0, dim <= 128; heads a multiple of kv_heads, at most 64
- * per kv_head; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold.
+ * per kv_head; kv_heads <= 1024; n_seq <= 1024.  total_q / total_k: rows that q / k and v hold.
  * workspace: 256-byte aligned, ane_attn_prompt_workspace_size bytes (which may be
  * 0), any contents, not shared by calls that may overlap. */
 size_t ane_attn_prompt_workspace_size(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t dim,
@@ -493,8 +493,8 @@ typedef struct ane_pages {
  * sees only those, read through the same pages for it alone.  Page numbers
  * outside the pool are read as page 0.  workspace: 256-byte aligned,
  * ane_attn_decode_workspace_size bytes, any contents, not shared by calls that
- * may overlap.  batch <= 1024; scale, dim, heads, kv_heads as for
- * ane_attn_prompt_dev. */
+ * may overlap.  batch <= 1024; heads <= 65535; else scale, dim, heads and
+ * kv_heads as for ane_attn_prompt_dev. */
 size_t ane_attn_decode_workspace_size(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim);
 int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, float scale,
                         const ane_rows* q, const ane_pages* pages, const int32_t* tables, uint32_t n_slots,

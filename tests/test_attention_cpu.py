@@ -262,3 +262,10 @@ def test_cache_takes_nothing_from_elsewhere(launches, device):
     with pytest.raises(ValueError):
         host.free(OnDevice(torch.zeros(1, dtype=torch.int32), -1))
     assert len(launches) == made
+
+
+def test_decode_most_heads():
+    """One head more than the join's grid takes is refused before anything is launched."""
+    assert decode(heads=65536, kv_heads=1024, q=rows(A, 64 * 65536), out=rows(A, 64 * 65536)) == INVALID
+    ok = decode(heads=65472, kv_heads=1023, q=rows(A, 64 * 65472), out=rows(A, 64 * 65472), batch=0)
+    assert ok == (0 if torch.cuda.is_available() else NO_DEVICE)
