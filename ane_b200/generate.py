@@ -99,7 +99,7 @@ class Generator:
         """One more token (row of x [n, hidden]) for each slot, the first `shared`
         tokens of all of them being the same (forks of one prompt).  Returns
         (output rows, granted); the row of a slot that was not granted is not
-        attended to and its output is to be dropped."""
+        in the cache and its output is to be dropped."""
         n = slots.numel()
         if ("one", n) not in self._ws:
             self._ws["one", n] = torch.ones(n, dtype=torch.int32, device=self.device)
@@ -126,6 +126,8 @@ def main(argv=None):
     a = ap.parse_args(argv)
     if not 1 <= a.children <= 15:
         ap.error("1 to 15 children")
+    if min(a.layers, a.prompt, a.steps) < 1:
+        ap.error("at least one layer, one token of the prompt and one step")
     tokens = a.prompt + a.steps
     gen = Generator(a.layers, slots=16, pages=16 * (tokens // 16 + 1), max_pages=tokens // 16 + 1)
     x, granted = gen.prompt(torch.randn(a.prompt, gen.hidden, device="cuda"),
@@ -137,7 +139,7 @@ def main(argv=None):
     begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     shared = a.prompt
     for step in range(a.steps):
-        if step == 1:
+        if step <= 1:  # the first step warms up, unless it is the only one
             begin.record()
         x, ok = gen.step(x, children, shared=shared)
     end.record()

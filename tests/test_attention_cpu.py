@@ -269,3 +269,13 @@ def test_decode_most_heads():
     assert decode(heads=65536, kv_heads=1024, q=rows(A, 64 * 65536), out=rows(A, 64 * 65536)) == INVALID
     ok = decode(heads=65472, kv_heads=1023, q=rows(A, 64 * 65472), out=rows(A, 64 * 65472), batch=0)
     assert ok == (0 if torch.cuda.is_available() else NO_DEVICE)
+
+
+@pytest.mark.parametrize("args", [["--steps", "0"], ["--prompt", "0"], ["--layers", "0"], ["--children", "0"],
+                                  ["--children", "16"], ["--steps", "-3"]])
+def test_generate_command_refusals(args, capsys):
+    from ane_b200 import generate
+
+    with pytest.raises(SystemExit) as e:
+        generate.main(args)
+    assert e.value.code == 2 and "error" in capsys.readouterr().err

@@ -99,3 +99,10 @@ def test_command_runs(ane, capsys):
 
     generate.main(["--layers", "1", "--prompt", "37", "--children", "3", "--steps", "3"])
     assert "3 continuations of 3 steps" in capsys.readouterr().out
+
+
+def test_command_runs_one_step(ane, capsys):
+    from ane_b200 import generate
+
+    generate.main(["--layers", "1", "--prompt", "1", "--children", "1", "--steps", "1"])
+    assert "1 continuations of 1 steps" in capsys.readouterr().out
