@@ -533,3 +533,94 @@ def test_single_rows_of_any_stride(ane):
     pool = lambda i: torch.as_strided(buf[i], (1, 8, 1, 64), (515, 64, 67, 1))  # noqa: E731  (one page, one head)
     out = ane.attn_decode(odd(0, 8), pool(1), pool(2).contiguous().view(1, 8, 1, 64), i32([[0]]), i32([7]))
     check_rows(out[0], F16, odd(0, 8)[0], pool(1)[0, :7, 0], pool(2)[0, :7, 0], 0.125, torch.full((8,), 7, device="cuda"))
+
+
+@pytest.mark.parametrize("lens,shared,heads,kv_heads,dim,page,dtype", [
+    ([4100 + b % 9 for b in range(38)] + [0, 100, 4095, 1, 2048], 4096, 32, 8, 64, 16, F16),  # prefix_kernel
+    ([1500, 700, 0, 1301, 1290, 1291], 1290, 8, 2, 128, 64, BF16),
+    ([70 + b for b in range(150)], 64, 8, 2, 64, 16, F16),
+])
+def test_decode_among_other_work(ane, lens, shared, heads, kv_heads, dim, page, dtype):
+    """The kernels of a call start before the ones in front of them have ended:
+    inputs that are written just before, overwritten just after, a workspace that the
+    next call takes over, on a side stream and in a graph."""
+    q, k, v, tables, lens_t, slots, want = decode_case(ane, lens, shared, heads, kv_heads, dim, page, dtype, seed=11)
+    swap = torch.arange(len(lens) - 1, -1, -1, device="cuda")
+    args = [(q, slots), (q[swap].contiguous(), slots[swap].contiguous())]
+    want = [want, ane.attn_decode(args[1][0], k, v, tables, lens_t, slots=args[1][1], shared=shared)]
+    ws = ane.attn_decode_workspace(len(lens), heads, kv_heads, dim)
+    qn, sn, ln = torch.empty_like(q), torch.empty_like(slots), torch.empty_like(lens_t)
+
+    def chain(stream=None):
+        got = []
+        for i in (0, 1, 1, 0):
+            qn.copy_(args[i][0])
+            sn.copy_(args[i][1])
+            ln.copy_(lens_t)
+            for t in range(2):
+                got.append((i, ane.attn_decode(qn, k, v, tables, ln, slots=sn, shared=shared, workspace=ws, stream=stream)))
+            qn.fill_(float("nan"))
+            ln.zero_()
+            sn.fill_(-1)
+        return got
+
+    def check(got):
+        torch.cuda.synchronize()
+        for i, out in got:
+            assert torch.equal(out, want[i])
+
+    ws.random_(0, 255)
+    check(chain())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ws.random_(0, 255)
+        got = chain(side)
+    check(got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(3):
+        for _, out in got:
+            out.zero_()
+        ws.random_(0, 255)
+        graph.replay()
+        check(got)
+
+
+@pytest.mark.parametrize("lq,lk", [([200, 90, 0, 7], [6000, 3000, 0, 7]), ([200, 64, 1], [200, 64, 1])])
+def test_prompt_among_other_work(ane, lq, lk):
+    """Items cut along the keys and whole ones: inputs that are written just before
+    and overwritten just after, a workspace that the next call takes over, in a graph."""
+    q, k, v, cq, ck, want = prompt_case(ane, lq, lk, 8, 2, 128, BF16, seed=12)
+    n = ane.lib.ane_attn_prompt_workspace_size(len(lq), 8, 2, 128, q.shape[0], k.shape[0])
+    assert (n > 0) == (max(lk) > 1000)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    c, d, qn, cn = i32(cq), i32(ck), torch.empty_like(q), i32(cq)
+
+    def chain():
+        got = []
+        for _ in range(3):
+            qn.copy_(q)
+            cn.copy_(c)
+            got += [ane.attn_prompt(qn, k, v, cn, d, workspace=ws) for _ in range(2)]
+            qn.fill_(float("nan"))
+            cn.zero_()
+        return got
+
+    def check(got):
+        torch.cuda.synchronize()
+        for out in got:
+            assert torch.equal(out[cq[0]:cq[-1]], want[cq[0]:cq[-1]])
+
+    ws.random_(0, 255)
+    check(chain())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(3):
+        for out in got:
+            out.zero_()
+        ws.random_(0, 255)
+        graph.replay()
+        check(got)
