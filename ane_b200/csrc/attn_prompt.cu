@@ -5,8 +5,8 @@
 // and dealt out to the blocks there and back again, so that every block's sum of
 // tiles is about the same without a queue in memory.
 //
-// Few items for the chip's 148 SMs (a block of a long prompt, some ragged
-// prompts): all items' key tiles are laid end to end and cut into equal spans,
+// Few long items for the chip's 148 SMs (a block of a prompt behind a long history):
+// all items' key tiles are laid end to end and cut into equal spans,
 // one per block.  An item cut by a boundary leaves unnormalised parts (m, l, o),
 // which join_kernel adds in the order of the keys.
 #include "attn_sm100.cuh"
@@ -369,17 +369,26 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     }
 }
 
-// Spans, or 0 for whole items.  The lengths are on the device; the host knows how
-// many items total_q tokens in n_seq pieces can make and how long a key line can
-// be.  From three items per SM dealing whole items out loses less than the parts
-// and their join cost (8 ragged prompts of up to 1531 tokens, 3 to 4 items per SM:
-// 46 us whole, 75 us as spans; 2 blocks of up to 1024 tokens behind 7681, 1.3 items
-// per SM and all of them long: 198 us whole, 169 us as spans; 2 prompts of 1000-4000
-// tokens, 8 heads, 1.6 items per SM of any length: 78 and 86).
-constexpr uint32_t kSpanKeys = 1024;
+// Spans, or 0 for whole items.  The lengths are on the device; the host knows their
+// means.  Where most keys are history, items are alike, and whole ones leave blocks
+// idle in their last wave: that has to outweigh the parts and their join (ten key
+// tiles a block) and that spans share K and V less (a fifth).  Without such a history
+// an item's length is anything up to the longest, and whole ones fill the blocks.
+// us whole and as spans, 32/8 heads x 128: 1 block of 1, 200, 500, 1000 tokens behind
+// 8000 115 and 49, 117 and 53, 140 and 84, 152 and 152; 4 of 1, 200, 500 behind 8000 127
+// and 56, 125 and 137, 232 and 294; 1 of 1, 200 behind 1000 21 and 29, 25 and 34; prompts
+// without history: 1 of 1000 tokens 25 and 39, of 2112 41 and 62, 4 of 500 23 and 41.
+// Over 926 calls of 1 to 8 sequences the choice costs 0.6 % of the better one's time on
+// average, 32 % at most (8/1 heads, 64 tokens behind 3000).
+constexpr int64_t kSpanKeys = 10 * kBigKeys;
 uint32_t spans_for(uint32_t n_seq, uint32_t group, uint32_t kv_heads, uint32_t total_q, uint32_t total_k) {
-    const uint64_t items = (uint64_t)(total_q / (2 * (kBigRows / group)) + n_seq) * kv_heads;
-    return items < 3 * kSpanBlocks && total_k >= kSpanKeys ? kSpanBlocks : 0;
+    if (n_seq == 0 || total_q == 0) return 0;
+    const int64_t queries = ceil_div(total_q, n_seq), keys = total_k / n_seq;
+    if (2 * queries > keys) return 0;
+    const int64_t items = (int64_t)ceil_div((size_t)queries, 2 * (kBigRows / group)) * n_seq * kv_heads;
+    const int64_t waves = (int64_t)ceil_div((size_t)items, kSpanBlocks);
+    // times 5 and the number of blocks
+    return (waves * 5 * kSpanBlocks - 6 * items) * (keys - queries / 2) > kSpanKeys * 5 * kSpanBlocks ? kSpanBlocks : 0;
 }
 
 template <typename T, int DP>

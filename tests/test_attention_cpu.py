@@ -279,3 +279,16 @@ def test_generate_command_refusals(args, capsys):
     with pytest.raises(SystemExit) as e:
         generate.main(args)
     assert e.value.code == 2 and "error" in capsys.readouterr().err
+
+
+def test_prompt_is_cut_where_a_history_is_long():
+    """Prompts without one are dealt out as whole items (cut ones take up to twice as
+    long), however few they are; a few blocks behind a long one are cut."""
+    f = L.ane_attn_prompt_workspace_size
+    for tokens in (17, 500, 1000, 2112, 5000, 16384):
+        for n in (1, 4, 9):
+            assert f(n, 32, 8, 128, tokens, tokens) == 0 and f(n, 8, 8, 64, tokens, tokens) == 0
+    assert f(4, 32, 8, 128, 800, 2000) == 0 and f(1, 32, 8, 128, 200, 1200) == 0
+    assert f(1, 32, 8, 128, 1, 8001) > 0 and f(2, 32, 8, 64, 1533, 1533 + 2 * 7681) > 0
+    assert f(0, 32, 8, 128, 0, 8000) == 0 and f(5, 32, 8, 128, 0, 8000) == 0
+    assert f(1024, 64, 1, 128, 2 ** 31 - 2 ** 17, 2 ** 31 - 2 ** 17) == 0

@@ -624,3 +624,18 @@ def test_prompt_among_other_work(ane, lq, lk):
         ws.random_(0, 255)
         graph.replay()
         check(got)
+
+
+@pytest.mark.parametrize("lq,lk,heads,kv_heads,dim,dtype", [
+    ([100, 513, 64], [9100, 8513, 9000], 8, 2, 128, BF16),
+    ([2000, 30], [1100, 19000], 4, 4, 128, F16),       # the first 900 queries see nothing
+    ([150, 90, 0, 70], [9150, 8000, 0, 15], 6, 2, 80, F16),
+    ([30] * 7, [9000 + 100 * i for i in range(7)], 16, 2, 64, F16),
+    ([260], [8200], 5, 1, 128, BF16),
+    ([700], [9000], 32, 8, 64, BF16),                  # two items and more a block
+])
+def test_prompt_long_history_cut_along_the_keys(ane, lq, lk, heads, kv_heads, dim, dtype):
+    n = ane.lib.ane_attn_prompt_workspace_size(len(lq), heads, kv_heads, dim, sum(lq) + 6, sum(lk) + 6)
+    assert n > 0  # parts
+    prompt_case(ane, lq, lk, heads, kv_heads, dim, dtype)
+    prompt_case(ane, lq, lk, heads, kv_heads, dim, dtype, out_dtype=F32, want_lse=False, seed=1)
