@@ -41,9 +41,14 @@ constexpr uint32_t kKept = 256;        // sequences whose slot and length stay i
 constexpr int kPagesAhead = 4;         // tiles whose page numbers are read ahead
 constexpr int kUnits = 4;              // units announced ahead
 constexpr int kUnitCost = 2;           // a unit's start and end cost about what two tiles do
-constexpr uint32_t kWholeTiles = 7;    // units of at most so many tiles are not cut (2 sequences x 32 heads in a
-                                       // graph, tiles a unit: whole and cut; 7: 12.3 and 12.3 us, 9: 14.3 and
-                                       // 12.3); a cut call costs the host a second launch
+// Units of at most so many tiles, as far as the width of the tables tells (the host
+// does not know the lengths), are not cut: a call then costs the host one launch, 2 us,
+// less, and the device goes through a unit's tiles one after another.  2 sequences x 32
+// heads, us in a graph, whole and cut: 3 tiles a unit 8.8 and 9.6, 5 10.1 and 10.2, 6
+// 10.9 and 10.1, 7 11.5 and 10.4; called from Python with other inputs each time: 7
+// tiles 12.4 and 14.4.  From 8 on the device's time shows there too (1 sequence of 510
+// in a graph: 11.5 and 10.4).
+constexpr uint32_t kWholeTiles = 7;
 
 struct Params {
     uint32_t batch, heads, kv_heads, group, dim, out_dtype;
