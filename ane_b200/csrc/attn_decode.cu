@@ -982,9 +982,11 @@ extern "C" int ane_attn_decode_dev(uint32_t dtype, uint32_t batch, uint32_t head
     p.shared = shared;
     // decode_kernel goes over the prefix once per unit of 16 rows.  The second time costs
     // little (L2), every further one a tile's time: prefix_kernel from where that
-    // makes eight tiles a block.  128 rows x 8 heads, 4096 shared: 29 us without it,
-    // 25 with it; 2048 shared: 23 and 25; 64 rows x 32 heads, 1024 shared: 33 and 36;
-    // 32 rows x 32 heads, 16384 shared: 70 and 86.
+    // makes eight tiles a block.  us without and with it: 128 rows x 8 heads behind 2048
+    // 23 and 24, behind 4096 29 and 26, behind 16384 64 and 35; 256 rows x 8 heads behind
+    // 1000 27 and 29, behind 2048 33 and 31; 64 rows x 32 heads behind 1000 35 and 36,
+    // behind 4096 54 and 50; 32 rows x 32 heads behind 16384 72 and 85.  Over 1056 calls
+    // of 2 to 256 sequences the choice costs 0.9 % of the better one's time on average.
     const uint32_t units = l.groups * l.subs;
     const uint64_t again = units > 2 ? (uint64_t)(units - 2) * kv_heads * ceil_div(shared, kTile) : 0;
     const bool big = again >= 8 * 2 * (uint64_t)kBigBlocks;
