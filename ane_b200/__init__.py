@@ -654,7 +654,9 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, out=None, out_dtype=None, 
     whole 16 bytes), sequence s at rows cu_q[s]:cu_q[s+1] of q and
     cu_k[s]:cu_k[s+1] of k and v (int32; cu_k defaults to cu_q).  The last query
     of a sequence sees its last key.  scale defaults to dim ** -0.5; out_dtype
-    may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp.
+    may be float32; lse (float32 [tokens, heads]) receives the log-sum-exp.  Rows
+    that belong to no sequence are not written (in a new result they hold anything);
+    within a sequence v has to be finite.
     workspace: a contiguous tensor of ane_attn_prompt_workspace_size bytes
     (default: a new one where the call needs any)."""
     T, heads, dim = q.shape

@@ -525,9 +525,9 @@ int ane_kv_fork_dev(const ane_kv_cache* cache, uint32_t n, const int32_t* parent
     if (n == 0) return ok();
     static std::atomic<uint64_t> done{0};
     if ((rc = allow_bits(fork_kernel, done))) return rc;
-    // Bound by what HBM takes in writes alone (3.9 TB/s here; a fill of 161 MB takes
-    // 45 us): 161 MB of part pages in 44 us with four blocks per SM (two 50, eight
-    // 57).  Reading a parent's page once for all its children changed nothing.
+    // 148 MB of part pages written and 18 read in 44 us with four blocks per SM (two 50,
+    // eight 57); a plain fill of those 148 MB takes 41.  Reading a parent's page once for
+    // all its children changed nothing.
     const size_t items = (size_t)n * (1 + 2 * p.layers);
     const uint32_t grid = (uint32_t)(items < (size_t)num_sms() * 4 ? items : (size_t)num_sms() * 4);
     rc = launch_pdl(fork_kernel, dim3(grid), dim3(kThreads), bits_bytes(p.pages), static_cast<cudaStream_t>(stream), p,

@@ -436,8 +436,9 @@ int ane_dense_fused_i8_noalloc_dev(uint32_t M, uint32_t N, uint32_t K, float sca
  * in the reference (its ggml backend leaves attention to ggml).
  *
  * Element types.  Queries, keys and values are 16-bit (F16 or BF16, one type
- * per call); scores, softmax statistics and sums are fp32; a result is rounded
- * once, to out_dtype (the inputs' type or F32). */
+ * per call); scores, softmax statistics and sums are fp32; a key's weight is
+ * rounded to the inputs' type before it is multiplied with V, whatever out_dtype
+ * is; a result is rounded once, to out_dtype (the inputs' type or F32). */
 #define ANE_DTYPE_F32 0u
 #define ANE_DTYPE_F16 1u
 #define ANE_DTYPE_BF16 2u
@@ -455,8 +456,8 @@ typedef struct ane_rows {
  * cu_q).  Its last query sees its last key: query i sees keys 0 .. i + lk - lq.
  * Query head h reads key/value head h / (heads / kv_heads):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][hk]) * v[j][hk]
- * A query that sees no key (lk < lq) gives 0 (and lse -inf).  Rows outside the
- * sequence are never part of a result, whatever they hold; inside it v has to be
+ * A query that sees no key (lk < lq) gives 0 (and lse -inf); rows of out and lse
+ * that belong to no sequence are not written.  Rows outside the sequence are never part of a result, whatever they hold; inside it v has to be
  * finite (a key that a query does not see yet has weight 0, and 0 * NaN is NaN).  lse (NULL to skip)
  * receives [total_q][heads] natural logarithms of the softmax sums.
  * scale > 0; dim % 8 == 0, dim <= 128; heads a multiple of kv_heads, at most 64
